@@ -251,6 +251,28 @@ int shk_qkv_store(void* qkv, int dtype, int n, int heads, int kv_heads, int head
                   const int32_t* token_seq, const int32_t* tables, int table_stride, void* k_pool,
                   void* v_pool, int page_size, int num_pages, int write_kv, void* stream);
 
+// A quantised cache (e4m3.h): keys and values as E4M3 codes, `scales` [num_pages, kv_heads, 2, page_size] bytes, the biased
+// exponents of a power of two per token and head, the keys' before the values'; pools of bytes in the layouts of shk_rope_kv_store.
+// In every call: tables is [num_seqs, table_stride]; a position below 0, or one whose page is beyond the tables or outside the
+// pool, is a token that is not there.
+// shk_rope_kv_store_e4m3: shk_rope_kv_store into such a cache, angles formed in float64; keys and values are quantised from float32.
+// Queries go to q_out, rows q_ld elements apart (qkv itself, q_ld its width: in place).  Tokens that are not there leave the pools alone.
+// shk_kv_read_e4m3: rows [n, kv_heads * head_dim] of `dtype` of the tokens (token_seq[t], positions[t]); NaN for one that is not there.
+// shk_attention_e4m3: shk_attention over such a cache (window, chunk; no cap, sinks or bias); scale > 0.  Keys that are not there
+// are not read; a query without any key gets zeros.
+int shk_rope_kv_store_e4m3(const void* qkv, int dtype, int n, int heads, int kv_heads, int head_dim, int rot_dim,
+                           const float* inv_freq, const int32_t* positions, const int32_t* token_seq, const int32_t* tables,
+                           int table_stride, int num_seqs, void* k_pool, void* v_pool, void* scales, int page_size, int num_pages,
+                           int write_kv, const float* parts, int splits, const float* bias, int pairing, int v_from_k,
+                           float magnitude, void* q_out, int q_ld, void* stream);
+int shk_kv_read_e4m3(void* k_out, void* v_out, int dtype, int n, int kv_heads, int head_dim, const int32_t* positions,
+                     const int32_t* token_seq, const int32_t* tables, int table_stride, int num_seqs, const void* k_pool,
+                     const void* v_pool, const void* scales, int page_size, int num_pages, void* stream);
+int shk_attention_e4m3(const void* q, int q_stride, void* out, int dtype, int n, int heads, int kv_heads, int head_dim,
+                       const int32_t* positions, const int32_t* token_seq, const int32_t* tables, int table_stride, int num_seqs,
+                       const void* k_pool, const void* v_pool, const void* scales, int page_size, int num_pages, int window,
+                       int chunk, float scale, void* stream);
+
 // 1 if the MFMA attention kernels take these shapes (head_dim a multiple of 32
 // up to 256, page_size a multiple of 16, at most 16 query heads per key/value
 // head, q rows 16-byte aligned); otherwise shk_attention serves them.

@@ -797,6 +797,112 @@ def _dist_bias(dist_bias, heads, who):
         raise KernelError(f"{who}: a distance bias must be contiguous float32 [heads ({heads}), rows]")
 
 
+# A quantised cache: keys and values as OCP E4M3 codes in the layouts of the bfloat16 cache, and for every token and head the
+# biased exponents of two powers of two, the keys' and the values' (csrc/e4m3.h says how they are chosen).
+E4M3 = torch.float8_e4m3fn
+
+
+def e4m3_scales_shape(pages: int, kv_heads: int, page_size: int) -> tuple:
+    """Exponent bytes (uint8) of a quantised cache: [pages, kv_heads, 2, page_size], the keys' before the values'."""
+    return (pages, kv_heads, 2, page_size)
+
+
+def _e4m3_cache(who, kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size) -> tuple:
+    """Arguments (tables, table_stride, num_seqs, pools, scales, page_size, num_pages) of a launcher, checked."""
+    pages = k_pool.shape[0]
+    if k_pool.dtype != E4M3 or v_pool.dtype != E4M3 or scales.dtype != torch.uint8:
+        raise KernelError(f"{who}: pools must be float8_e4m3fn and scales uint8, got {k_pool.dtype}, {v_pool.dtype}, {scales.dtype}")
+    if k_pool.shape != key_pool_shape(pages, kv_heads, page_size, head_dim):
+        raise KernelError(f"{who}: key pool must be {list(key_pool_shape('pages', kv_heads, page_size, head_dim))}, "
+                          f"got {tuple(k_pool.shape)}")
+    if v_pool.shape != (pages, kv_heads, head_dim, page_size) or scales.shape != (pages, kv_heads, 2, page_size):
+        raise KernelError(f"{who}: value pool must be [{pages}, {kv_heads}, {head_dim}, {page_size}] and scales "
+                          f"[{pages}, {kv_heads}, 2, {page_size}], got {tuple(v_pool.shape)} and {tuple(scales.shape)}")
+    if not (k_pool.is_contiguous() and v_pool.is_contiguous() and scales.is_contiguous() and tables.is_contiguous()):
+        raise KernelError(f"{who}: pools, scales and tables must be contiguous")
+    if tables.dim() != 2:
+        raise KernelError(f"{who}: tables must be [sequences, blocks]")
+    if k_pool.data_ptr() % 16 or v_pool.data_ptr() % 16 or scales.data_ptr() % 16:
+        raise KernelError(f"{who}: pools and scales must be 16-byte aligned")
+    return (_dev(tables, "tables", torch.int32), tables.shape[1], tables.shape[0], _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool"),
+            _dev(scales, "scales"), page_size, pages)
+
+
+def _step_rows(who, n, *arrays) -> None:
+    for a in arrays:
+        if a.dim() != 1 or a.shape[0] < n or not a.is_contiguous():
+            raise KernelError(f"{who}: the call has {n} rows, and positions and token_seq must be contiguous with one number for each")
+
+
+def rope_kv_store_e4m3(qkv, heads, kv_heads, head_dim, rot_dim, inv_freq, positions, token_seq, tables, k_pool, v_pool, scales,
+                       page_size, write_kv=True, split_sum=None, adjacent_pairs: bool = False, values_from_keys: bool = False,
+                       magnitude: float = 1.0, q_out=None) -> None:
+    """rope_kv_store() into a quantised cache: queries and keys are rotated, keys and values of every token and head are divided by a
+    power of two of their own and rounded to E4M3, and that power's biased exponent goes to `scales`.  Angles are formed in
+    float64.  q_out: rows [n, heads * head_dim] of qkv's dtype with unit inner stride that receive the queries (None: qkv's own query columns, in
+    place; all of qkv's other columns stay as they are)."""
+    n = qkv.shape[0]
+    width = (heads + (1 if values_from_keys else 2) * kv_heads) * head_dim
+    if qkv.dim() != 2 or not qkv.is_contiguous() or qkv.shape[1] != width:
+        raise KernelError("rope_kv_store_e4m3: qkv must be contiguous [n, (heads + 2 kv_heads) head_dim] "
+                          "(heads + kv_heads with values_from_keys)")
+    if q_out is None:
+        q_out = qkv
+    elif q_out.dim() != 2 or q_out.stride(1) != 1 or q_out.shape != (n, heads * head_dim) or q_out.dtype != qkv.dtype:
+        raise KernelError("rope_kv_store_e4m3: q_out must be rows [n, heads * head_dim] of qkv's dtype with unit inner stride")
+    if rot_dim and (inv_freq is None or inv_freq.numel() < rot_dim // 2 or not inv_freq.is_contiguous()):
+        raise KernelError(f"rope_kv_store_e4m3: a rotation of {rot_dim} elements needs {rot_dim // 2} frequencies")
+    parts, splits, bias = None, 0, None
+    if split_sum is not None:
+        parts, bias = split_sum.parts, split_sum.bias
+        splits = parts.shape[0]
+        if tuple(parts.shape[1:]) != tuple(qkv.shape) or parts.dtype != torch.float32 or not parts.is_contiguous():
+            raise KernelError("rope_kv_store_e4m3: partial sums must be contiguous float32 [splits, n, width]")
+        if bias is not None and (bias.numel() != width or not bias.is_contiguous()):
+            raise KernelError("rope_kv_store_e4m3: the partial sums' bias must be contiguous [width]")
+    cache = (None, 0, 0, None, None, None, page_size, 0)
+    if write_kv:
+        cache = _e4m3_cache("rope_kv_store_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size)
+        _step_rows("rope_kv_store_e4m3", n, positions, token_seq)
+    else:
+        _step_rows("rope_kv_store_e4m3", n, positions)
+    check(load().shk_rope_kv_store_e4m3(
+        _dev(qkv, "qkv"), dtype_code(qkv.dtype), n, heads, kv_heads, head_dim, rot_dim,
+        _dev(inv_freq, "inv_freq", torch.float32) if rot_dim else None, _dev(positions, "positions", torch.int32),
+        _dev(token_seq, "token_seq", torch.int32) if write_kv else None, *cache, int(bool(write_kv)),
+        None if parts is None else _dev(parts, "parts"), splits, None if bias is None else _dev(bias, "bias", torch.float32),
+        int(bool(adjacent_pairs)), int(bool(values_from_keys)), float(magnitude), _dev(q_out, "q_out"), q_out.stride(0), _stream()))
+
+
+def kv_read_e4m3(k_out, v_out, kv_heads, head_dim, positions, token_seq, tables, k_pool, v_pool, scales, page_size) -> None:
+    """Rows [n, kv_heads * head_dim] (float32 or bfloat16, which holds the values exactly) of the cached keys and values of the
+    tokens at positions[t] of sequences token_seq[t]; NaN for a token that the tables do not have."""
+    n = k_out.shape[0]
+    if k_out.shape != (n, kv_heads * head_dim) or v_out.shape != k_out.shape or v_out.dtype != k_out.dtype \
+            or not (k_out.is_contiguous() and v_out.is_contiguous()):
+        raise KernelError("kv_read_e4m3: k_out and v_out must be contiguous [n, kv_heads * head_dim] of one dtype")
+    _step_rows("kv_read_e4m3", n, positions, token_seq)
+    check(load().shk_kv_read_e4m3(
+        _dev(k_out, "k_out"), _dev(v_out, "v_out"), dtype_code(k_out.dtype), n, kv_heads, head_dim,
+        _dev(positions, "positions", torch.int32), _dev(token_seq, "token_seq", torch.int32),
+        *_e4m3_cache("kv_read_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size), _stream()))
+
+
+def attention_e4m3(q, out, heads, kv_heads, head_dim, positions, token_seq, tables, k_pool, v_pool, scales, page_size, window, scale,
+                   chunk=None) -> None:
+    """attention() over a quantised cache, any sizes: q [n, >= heads * head_dim] rows of float32 or bfloat16, out [n, heads * head_dim]."""
+    _rows(q, "attention_e4m3 q")
+    n = q.shape[0]
+    if q.shape[1] < heads * head_dim or out.shape != (n, heads * head_dim) or not out.is_contiguous() or out.dtype != q.dtype:
+        raise KernelError("attention_e4m3: out must be contiguous [n, heads * head_dim] of q's dtype, q at least as wide")
+    _step_rows("attention_e4m3", n, positions, token_seq)
+    check(load().shk_attention_e4m3(
+        _dev(q, "q"), q.stride(0), _dev(out, "out"), dtype_code(q.dtype), n, heads, kv_heads, head_dim,
+        _dev(positions, "positions", torch.int32), _dev(token_seq, "token_seq", torch.int32),
+        *_e4m3_cache("attention_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size), int(window or 0),
+        int(chunk or 0), float(scale), _stream()))
+
+
 def qkv_store(qkv, heads, kv_heads, head_dim, v_dim, positions, token_seq, tables, k_pool, v_pool, page_size,
               q_temperature=None, v_norm_eps=None, write_kv=True, qk_norm_eps=None, q_weight=None, k_weight=None,
               has_kv=True) -> None:

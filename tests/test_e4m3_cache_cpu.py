@@ -1,0 +1,67 @@
+"""What the launchers of the quantised cache refuse (nothing is launched), and the 64-bit oracle against torch's conversion."""
+
+import pytest
+import torch
+
+from . import e4m3_plain as plain
+
+
+def test_the_oracle_rounds_as_the_type_does():
+    codes = torch.arange(256, dtype=torch.uint8).view(plain.E4M3).float().double()
+    codes = codes[codes.isfinite()]
+    assert codes.numel() == 254
+    assert torch.equal(plain.rounded(codes), codes)
+    x = torch.randn(100000, generator=torch.Generator().manual_seed(1), dtype=torch.float64) * 50
+    x = torch.cat([x, x * 2.0 ** -10, (codes[1:] + codes[:-1]) / 2]).clamp(-448, 448)
+    assert torch.equal(plain.rounded(x), x.float().to(plain.E4M3).double())
+
+
+def test_the_oracle_s_exponents():
+    x = torch.tensor([[0.0], [448.0], [449.0], [224.0], [1e-300], [1e300], [448 * 2.0 ** 119]], dtype=torch.float64)
+    assert plain.exponents(x).tolist() == [-117, 0, 1, -1, -117, 119, 119]
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from shrike_amd.kernels.lib import load
+
+    return load()
+
+
+def refused(lib, name, args, part):
+    assert getattr(lib, name)(*args) != 0
+    assert part in lib.shk_last_error().decode()
+
+
+def test_refusals_before_any_launch(lib):
+    P = None
+
+    def store(dtype=1, n=4, heads=4, kv=2, dim=64, rot=64, ps=16, pages=9, stride=3, seqs=2, splits=0, pairing=0, q_ld=512, bias=P):
+        return (P, dtype, n, heads, kv, dim, rot, P, P, P, P, stride, seqs, P, P, P, ps, pages, 1, P, splits, bias, pairing, 0, 1.0, P,
+                q_ld, P)
+
+    name = "shk_rope_kv_store_e4m3"
+    assert getattr(lib, name)(*store(n=0)) == 0
+    for args, part in ((store(dtype=2), "dtype"), (store(n=-1), "n=-1"), (store(dim=257), "head_dim=257"), (store(rot=66), "rot_dim"),
+                       (store(rot=63), "rot_dim"), (store(pairing=2), "pairing"), (store(q_ld=255), "queries"),
+                       (store(splits=2), "parts"), (store(heads=0), "heads=0"), (store(), "null pointer")):
+        refused(lib, name, args, part)
+
+    def read(dtype=1, n=4, kv=2, dim=64, ps=16, pages=9, stride=3, seqs=2):
+        return (P, P, dtype, n, kv, dim, P, P, P, stride, seqs, P, P, P, ps, pages, P)
+
+    name = "shk_kv_read_e4m3"
+    assert getattr(lib, name)(*read(n=0)) == 0
+    for args, part in ((read(dtype=5), "dtype"), (read(kv=0), "kv_heads=0"), (read(ps=0), "page_size=0"), (read(pages=0), "num_pages=0"),
+                       (read(), "null pointer")):
+        refused(lib, name, args, part)
+
+    def attend(dtype=1, n=4, heads=4, kv=2, dim=64, q_ld=256, ps=16, pages=9, scale=0.1):
+        return (P, q_ld, P, dtype, n, heads, kv, dim, P, P, P, 3, 2, P, P, P, ps, pages, 0, 0, scale, P)
+
+    name = "shk_attention_e4m3"
+    assert getattr(lib, name)(*attend(n=0)) == 0
+    for args, part in ((attend(dtype=3), "dtype"), (attend(heads=3), "multiple"), (attend(dim=300), "head_dim"), (attend(q_ld=255), "q_stride"),
+                       (attend(ps=0), "page_size=0"), (attend(scale=0.0), "positive"), (attend(scale=float("nan")), "positive"),
+                       (attend(n=70000), "65535"), (attend(), "null pointer")):
+        refused(lib, name, args, part)
