@@ -273,6 +273,22 @@ int shk_attention_e4m3(const void* q, int q_stride, void* out, int dtype, int n,
                        const void* k_pool, const void* v_pool, const void* scales, int page_size, int num_pages, int window,
                        int chunk, float scale, void* stream);
 
+// The same on the matrix units for bfloat16, where shk_attention_e4m3_supports_mfma says so (head_dim a multiple of 32 up to 256,
+// page_size of 16, up to 128 query heads a key/value head, q rows 16-byte aligned).
+// shk_attention_decode_e4m3: sequence s has one query token, row s of q, at positions[s]; nsplit > 1 workgroups share its keys.
+// shk_attention_prefill_e4m3: rows first_seq .. n - 1 of q and out are the new tokens of sequences first_seq .. first_seq +
+// num_seqs - 1 (those before have a token each): rows cu_q[s] .. cu_q[s + 1], at the end of ctx_lens[s] tokens.  Other rows stay.
+// partial with nsplit > 1 (up to 64): rows * heads * nsplit * (head_dim + 2) floats.
+int shk_attention_e4m3_supports_mfma(int heads, int kv_heads, int head_dim, int page_size, int q_stride);
+int shk_attention_decode_e4m3(const void* q, int q_stride, void* out, int num_seqs, int heads, int kv_heads, int head_dim,
+                              const int32_t* positions, const int32_t* tables, int table_stride, int table_rows, const void* k_pool,
+                              const void* v_pool, const void* scales, int page_size, int num_pages, int window, int chunk, float scale,
+                              float* partial, int nsplit, void* stream);
+int shk_attention_prefill_e4m3(const void* q, int q_stride, void* out, int n, int first_seq, int num_seqs, int heads, int kv_heads,
+                               int head_dim, const int32_t* cu_q, const int32_t* ctx_lens, const int32_t* tables, int table_stride,
+                               int table_rows, const void* k_pool, const void* v_pool, const void* scales, int page_size,
+                               int num_pages, int window, int chunk, float scale, float* partial, int nsplit, void* stream);
+
 // 1 if the MFMA attention kernels take these shapes (head_dim a multiple of 32
 // up to 256, page_size a multiple of 16, at most 16 query heads per key/value
 // head, q rows 16-byte aligned); otherwise shk_attention serves them.

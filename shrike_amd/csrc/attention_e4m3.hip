@@ -3,6 +3,8 @@
 //
 // attention_e4m3_kernel: any head size up to 256, any page size and group, float32 or bfloat16 queries; one workgroup per
 // (token, head).  What the kernels on the matrix units do not take.
+// attention_decode_e4m3_kernel, attention_portion_e4m3_kernel: bfloat16 queries, head sizes in multiples of 32, pages in
+// multiples of 16.
 #include "api.h"
 #include "common.h"
 #include "e4m3.h"
@@ -10,6 +12,11 @@
 
 namespace shk {
 
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMaxShares = 64;  // workgroups that share a query's keys: a lane of the kernel that joins them each
 constexpr int kGeneralThreads = 256, kGeneralDim = 256;
 
 // Keys in runs of 256 from the query's first key on, a thread per key for its score, a thread per (part of the run, element)
@@ -74,6 +81,591 @@ __global__ void __launch_bounds__(kGeneralThreads)
   }
 }
 
+// ------------------------------------------------------------------- decode
+// One query token per sequence on the matrix units: grid (key/value head x tiles of 16 of its query heads, sequence, share of the
+// keys), four wavefronts that take the share's chunks of 64 keys by turns.  Products are formed transposed (S^T = K Q^T,
+// O^T += V^T P^T): lane (j, g) = (lane % 16, lane / 16) owns query head j throughout.
+//
+// A chunk is four blocks of 16 keys, none of which crosses a page (page sizes are multiples of 16).  Row R = 4 b + i of score
+// tile t is key 16 b + 4 t + i, so that lane (j, g) ends up with the scores of the sixteen keys of block g: their values' codes are
+// 16 bytes of a page for every element, one load, and are its operand of the second product as they come.  Of its keys' rows a
+// lane loads 16 bytes too, of two slabs of 32 elements at a time (the order of the elements within a product is free as long
+// as both operands agree); a head size with an odd number of slabs takes its last one in pieces of 8.
+// Keys become bfloat16 with their power of two, values without: theirs joins the weight, before that is rounded to bfloat16.
+template <int D>
+struct KeyBlock {
+  static constexpr int kPairs = D / 64, kOdd = D / 32 % 2;
+  u32x4 pair[kPairs ? kPairs : 1];
+  uint2 odd;
+};
+template <int D>
+struct CodeChunk {
+  KeyBlock<D> k[4];
+  u32x4 v[D / 16];
+  u32x4 k_exp, v_exp;  // exponent bytes of the sixteen keys of block j / 4, of block g
+};
+
+__device__ __forceinline__ bf16x8 bf16_of_codes(uint32_t lo, uint32_t hi, float unit) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(lo), unit, false);
+  const auto b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(lo), unit, true);
+  const auto c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(hi), unit, false);
+  const auto d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(hi), unit, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+template <int D, int WAVES>
+__global__ void __launch_bounds__(WAVES* kWave)
+    attention_decode_e4m3_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict__ out, int heads, int head_tiles,
+                                 const int32_t* __restrict__ positions, const int32_t* __restrict__ tables, int table_stride,
+                                 const uint8_t* __restrict__ k_pool, const uint8_t* __restrict__ v_pool,
+                                 const uint8_t* __restrict__ scales, int kv_heads, int page_size, uint32_t page_magic, int num_pages,
+                                 int window, int block, float scale, float* __restrict__ partial, int nsplit) {
+  constexpr int kStep = 64 * WAVES;  // keys between two chunks of one wavefront
+  constexpr int kPairs = D / 64, kOdd = D / 32 % 2;
+  __shared__ float m_lds[WAVES][16], l_lds[WAVES][16];
+  __shared__ float4 o_lds[WAVES][D / 16][kWave];
+  const int kvh = blockIdx.x / head_tiles, seq = blockIdx.y, z = blockIdx.z;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, j = lane % 16, g = lane / 16;
+  const int group = heads / kv_heads;
+  const int first_head = kvh * group + blockIdx.x % head_tiles * 16;  // of this workgroup's tile
+  const int tile_heads = min(16, kvh * group + group - first_head);
+  const PageDiv pd{page_size, page_magic};
+  const int pos = positions[seq], lo = first_key(pos, window, block);
+  const int first = lo & ~63;
+  const int chunks = pos < 0 ? 0 : (pos - first) / 64 + 1;
+  const int per = (chunks + nsplit - 1) / nsplit;
+  const int key_begin = first + z * per * 64 + wave * 64;
+  int key_end = first + (z + 1) * per * 64;
+  if (key_end > pos + 1) key_end = pos + 1;
+
+  // softmax state of head j, in base-2 logarithms; `l` is this lane's share of the sum until the end
+  float m = -INFINITY, l = 0.f;
+  f32x4 o[D / 16];  // element db * 16 + 4 * g + r of head j
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (key_begin < key_end) {
+    // the queries in the order of the keys' elements; lanes without a head take the tile's first again and are dropped in the end
+    bf16x8 qf[D / 32];
+    {
+      const bf16* row = q + static_cast<size_t>(seq) * q_stride + static_cast<size_t>(first_head + (j < tile_heads ? j : 0)) * D;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const bf16* from = row + (2 * i + g / 2) * 32 + g % 2 * 16;
+        qf[2 * i] = *reinterpret_cast<const bf16x8*>(from);
+        qf[2 * i + 1] = *reinterpret_cast<const bf16x8*>(from + 8);
+      }
+      if (kOdd) qf[D / 32 - 1] = *reinterpret_cast<const bf16x8*>(row + kPairs * 64 + g * 8);
+    }
+    const float scale2 = scale * 1.4426950408889634f;
+    const int32_t* table = tables + static_cast<size_t>(seq) * table_stride;
+    const size_t row_bytes = static_cast<size_t>(page_size) * D;
+
+    // The page of the block of 16 keys that holds key `kb` (of the nearest one that the query reads), and its first slot there.
+    auto clamped_block = [&](int kb) {
+      kb = kb < (lo & ~15) ? lo & ~15 : kb;
+      return kb > pos ? pos & ~15 : kb;
+    };
+    auto page_of = [&](int kb) {
+      const int entry = pd.div(clamped_block(kb));
+      const int page = table[entry < table_stride ? entry : table_stride - 1];
+      return page >= 0 && page < num_pages ? page : 0;  // (an id outside the pool is never followed)
+    };
+    struct Pages {
+      int k, v;
+    };
+    auto find = [&](int kb) { return Pages{page_of(kb + j / 4 * 16), page_of(kb + g * 16)}; };
+    auto fetch = [&](CodeChunk<D>& c, int kb, Pages at) {
+      const int k_slot = pd.mod(clamped_block(kb + j / 4 * 16)), v_slot = pd.mod(clamped_block(kb + g * 16));
+      const size_t k_part = static_cast<size_t>(at.k) * kv_heads + kvh, v_part = static_cast<size_t>(at.v) * kv_heads + kvh;
+      const uint8_t* key = k_pool + k_part * row_bytes + static_cast<size_t>(k_slot + j % 4) * 32;
+      const uint8_t* pair = key + static_cast<size_t>(g / 2) * page_size * 32 + g % 2 * 16;
+      const uint8_t* odd = key + static_cast<size_t>(2 * kPairs) * page_size * 32 + g * 8;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+          c.k[t].pair[i] = *reinterpret_cast<const u32x4*>(pair + t * 128 + static_cast<size_t>(i) * page_size * 64);
+        if (kOdd) c.k[t].odd = *reinterpret_cast<const uint2*>(odd + t * 128);
+      }
+      const uint8_t* value = v_pool + v_part * row_bytes + static_cast<size_t>(j) * page_size + v_slot;
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) c.v[db] = *reinterpret_cast<const u32x4*>(value + static_cast<size_t>(db) * 16 * page_size);
+      c.k_exp = *reinterpret_cast<const u32x4*>(scales + k_part * 2 * page_size + k_slot);
+      c.v_exp = *reinterpret_cast<const u32x4*>(scales + (v_part * 2 + 1) * page_size + v_slot);
+    };
+
+    auto attend_chunk = [&](const CodeChunk<D>& c, int kb, auto edge_tag) {
+      constexpr bool edge = decltype(edge_tag)::value;
+      f32x4 s[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        // this lane's row of the tile is key 4 t + j % 4 of block j / 4
+        const float unit = __uint_as_float((c.k_exp[t] >> (j % 4 * 8) & 0xffu) << 23);
+        s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          const u32x4 w = c.k[t].pair[i];
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(w[0], w[1], unit), qf[2 * i], s[t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(w[2], w[3], unit), qf[2 * i + 1], s[t], 0, 0, 0);
+        }
+        if (kOdd)
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(c.k[t].odd.x, c.k[t].odd.y, unit), qf[D / 32 - 1], s[t], 0, 0, 0);
+      }
+      // this lane's keys are kb + 16 g + e, e = 4 t + r
+      const int g0 = kb + g * 16;
+      float sc[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = s[e / 4][e % 4] * scale2;
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (g0 + e > pos || g0 + e < lo) sc[e] = -INFINITY;
+      }
+      float mx = max3(sc[0], sc[1], sc[2]);
+#pragma unroll
+      for (int e = 3; e < 15; e += 2) mx = max3(mx, sc[e], sc[e + 1]);
+      mx = lanes4_max(fmaxf(mx, sc[15]));
+      const float m_new = fmaxf(m, mx);
+      const float m_safe = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m - m_safe);
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      bf16x8 pf[2];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float p = __builtin_amdgcn_exp2f(sc[e] - m_safe);
+        sum[e % 4] += p;
+        float unit = __uint_as_float((c.v_exp[e / 4] >> (e % 4 * 8) & 0xffu) << 23);
+        // a slot that the query does not read may hold any byte: infinity, and 0 times that would be NaN
+        if (edge && (g0 + e > pos || g0 + e < lo)) unit = 0.f;
+        pf[e / 8][e % 8] = static_cast<__bf16>(p * unit);
+      }
+      l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+      m = m_new;
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db) o[db] *= alpha;
+      }
+      u32x4 keep = {~0u, ~0u, ~0u, ~0u};  // and its value any code, NaN among them
+      if (edge) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t bits = 0;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) bits |= g0 + 4 * w + b > pos || g0 + 4 * w + b < lo ? 0u : 0xffu << (8 * b);
+          keep[w] = bits;
+        }
+      }
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) {
+        u32x4 v = c.v[db];
+        if (edge) v &= keep;
+        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(v[0], v[1], 1.f), pf[0], o[db], 0, 0, 0);
+        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(v[2], v[3], 1.f), pf[1], o[db], 0, 0, 0);
+      }
+    };
+    auto attend = [&](const CodeChunk<D>& c, int kb) {
+      if (kb + 63 > pos || kb < lo)  // wave-uniform
+        attend_chunk(c, kb, EdgeTag<true>{});
+      else
+        attend_chunk(c, kb, EdgeTag<false>{});
+    };
+
+    // One chunk's loads are in flight while the chunk before is computed, and the pages of the one after; every step issues the
+    // same loads (past the end the last chunk's again), so that the compiler can count them.
+    const int last = key_begin + (key_end - 1 - key_begin) / kStep * kStep;
+    auto clamped = [&](int kb) { return kb < last ? kb : last; };
+    CodeChunk<D> buf[2];
+    fetch(buf[0], key_begin, find(key_begin));
+    Pages next = find(clamped(key_begin + kStep));
+    for (int kb0 = key_begin; kb0 < key_end; kb0 += 2 * kStep) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int kb = kb0 + kStep * u;
+        if (kb >= key_end) break;
+        fetch(buf[1 - u], clamped(kb + kStep), next);
+        next = find(clamped(kb + 2 * kStep));
+        attend(buf[u], kb);
+      }
+    }
+    l = lanes4_sum(l);
+  }
+
+  // ---- the wavefronts' results become one: common maximum, sums in wavefront order
+  if (g == 0) {
+    m_lds[wave][j] = m;
+    l_lds[wave][j] = l;
+  }
+  __syncthreads();
+  float m_all = m_lds[0][j];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) m_all = fmaxf(m_all, m_lds[w][j]);
+  const float m_ref = m_all == -INFINITY ? 0.f : m_all;
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) l += l_lds[w][j] * __builtin_amdgcn_exp2f(m_lds[w][j] - m_ref);  // 2^-inf = 0: nothing seen
+  const float mine = __builtin_amdgcn_exp2f(m - m_ref);
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db) o_lds[wave][db][lane] = make_float4(o[db][0] * mine, o[db][1] * mine, o[db][2] * mine, o[db][3] * mine);
+  __syncthreads();
+  if (j >= tile_heads) return;
+  const size_t head = static_cast<size_t>(seq) * heads + first_head + j;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // (a query that reads no key: zeros)
+#pragma unroll
+  for (int i = 0; i < (D / 16 + WAVES - 1) / WAVES; ++i) {
+    const int db = wave + i * WAVES;
+    if (D / 16 % WAVES && db >= D / 16) break;
+    float4 v = o_lds[0][db][lane];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+      const float4 x = o_lds[w][db][lane];
+      v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+    }
+    if (nsplit == 1) {
+      uint2 packed;
+      packed.x = bf16_bits(v.x * inv) | static_cast<uint32_t>(bf16_bits(v.y * inv)) << 16;
+      packed.y = bf16_bits(v.z * inv) | static_cast<uint32_t>(bf16_bits(v.w * inv)) << 16;
+      *reinterpret_cast<uint2*>(out + head * D + 4 * g + db * 16) = packed;
+    } else {
+      *reinterpret_cast<float4*>(partial + (head * nsplit + z) * D + 4 * g + db * 16) = v;
+    }
+  }
+  // partial: O [row][share][D], then (maximum, sum) [row][share][2]
+  if (nsplit > 1 && wave == 0 && g == 0)
+    *reinterpret_cast<float2*>(partial + static_cast<size_t>(gridDim.y) * heads * nsplit * D + (head * nsplit + z) * 2) =
+        make_float2(m_all, l);
+}
+
+// out[row] = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z, shares in order: a wavefront per row (a token's head), lane z with share
+// z's weight.
+template <int D>
+__global__ void __launch_bounds__(kWave) merge_e4m3_kernel(const float* __restrict__ partial, bf16* __restrict__ out, int nsplit) {
+  constexpr int kBatch = 8, NE = (D + kWave - 1) / kWave;
+  const size_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  const float* src = partial + row * nsplit * D;
+  float2 mine = make_float2(-INFINITY, 0.f);
+  if (lane < nsplit) mine = *reinterpret_cast<const float2*>(partial + static_cast<size_t>(gridDim.x) * nsplit * D + (row * nsplit + lane) * 2);
+  float x[kBatch][NE];
+  auto fetch = [&](int z0) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+      for (int e = 0; e < NE; ++e) x[u][e] = src[static_cast<size_t>(min(z0 + u, nsplit - 1)) * D + min(lane + e * kWave, D - 1)];
+  };
+  fetch(0);
+  const float mx = wave_max(mine.x);
+  const float w = mine.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine.x - mx);
+  float den = 0.f, acc[NE];
+#pragma unroll
+  for (int e = 0; e < NE; ++e) acc[e] = 0.f;
+  for (int z0 = 0; z0 < nsplit; z0 += kBatch) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const float wz = z0 + u < nsplit ? __shfl(w, z0 + u, kWave) : 0.f;
+      den += z0 + u < nsplit ? __shfl(w * mine.y, z0 + u, kWave) : 0.f;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) acc[e] += wz * x[u][e];
+    }
+    if (z0 + kBatch < nsplit) fetch(z0 + kBatch);
+  }
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+  for (int e = 0; e < NE; ++e)
+    if (lane + e * kWave < D) out[row * D + lane + e * kWave] = from_float<bf16>(acc[e] * inv);
+}
+
+// ------------------------------------------------------------------ portions
+// Runs of new tokens over the pages that hold what came before and the run itself.  A row is one query of one head; the heads that
+// share a key/value head read the same keys, so a workgroup takes all of them for a run of queries: 32 rows a wavefront, whatever
+// the heads of a group.  Products as above with v_mfma_f32_32x32x16_bf16: a lane owns half of a row's scores, and the weights go
+// from one product into the next without leaving it.
+//
+// Chunks of 64 keys.  Codes come from the pages into registers a chunk ahead and go to LDS as bfloat16 values, each of them
+// converted once for all rows of the workgroup:
+//   keys    [block of 16][32 elements] units of 1 KiB, 64 bytes a key: piece c of 16 bytes of a key at place c ^ (key / 4),
+//   values  [block of 16][32 elements] units, 32 bytes an element: piece c at place c ^ (element / 8 % 2),
+// so that the lanes that LDS serves together meet no bank conflicts.  Row 8 a + 4 h + r of a score tile is key 16 (a / 2) + 8 h +
+// 4 (a % 2) + r of its 32: a lane's scores are then, in order, the eight keys that it brings to each step of the second product.
+//
+// The workgroups find their queries themselves, a sequence's last queries (which read the most keys) first, so a step needs no
+// lists from the host.
+struct PortionArgs {
+  const bf16* q;
+  bf16* out;
+  const int32_t *cu_q, *ctx_lens, *tables;
+  const uint8_t *k_pool, *v_pool, *scales;
+  float* partial;
+  int n, q_stride, heads, kv_heads, queries, first_seq, num_seqs, table_stride, page_size, num_pages, window, block, nsplit;
+  uint32_t page_magic;
+  float scale;
+};
+
+template <int D, int WAVES>
+__global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attention_portion_e4m3_kernel(PortionArgs a) {
+  constexpr int KS = D / 16, DB = D / 32;
+  constexpr int kThreads = WAVES * kWave, kSide = 64 * D * 2;  // bytes of a chunk's keys as bfloat16
+  constexpr int kPieces = 4 * D;                               // of 16 codes of its keys (as many of its values)
+  constexpr int kPer = (2 * kPieces + kThreads - 1) / kThreads;
+  __shared__ u32x4 mem[2][2 * kSide / 16];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int col = lane % 32, half = lane / 32;
+  const PageDiv pd{a.page_size, a.page_magic};
+  const int z = blockIdx.x % a.nsplit, kvh = blockIdx.x / a.nsplit % a.kv_heads;
+
+  // ---- this workgroup's sequence and first query
+  int seq = -1, q0 = 0;
+  {
+    int left = blockIdx.x / (a.nsplit * a.kv_heads);
+    for (int base = 0; base < a.num_seqs; base += kWave) {
+      const int i = base + lane;
+      int runs = 0;
+      if (i < a.num_seqs) runs = (a.cu_q[a.first_seq + i + 1] - a.cu_q[a.first_seq + i] + a.queries - 1) / a.queries;
+      int upto = runs;
+#pragma unroll
+      for (int off = 1; off < kWave; off <<= 1) {
+        const int below = __shfl_up(upto, off, kWave);
+        if (lane >= off) upto += below;
+      }
+      const uint64_t past = __builtin_amdgcn_ballot_w64(upto > left);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        seq = a.first_seq + base + at;
+        q0 = (__shfl(upto, at, kWave) - 1 - left) * a.queries;
+        break;
+      }
+      left -= __shfl(upto, kWave - 1, kWave);
+    }
+    if (seq < 0) return;  // (there are at most as many runs as workgroups)
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    q0 = __builtin_amdgcn_readfirstlane(q0);
+  }
+  const int group = a.heads / a.kv_heads;
+  const int tok0 = a.cu_q[seq], q_len = min(a.cu_q[seq + 1], a.n) - tok0;
+  if (tok0 < a.first_seq || q0 >= q_len) return;  // (ranges that are not the rows' are a mistake of the caller's, never followed)
+  const int start = a.ctx_lens[seq] - (a.cu_q[seq + 1] - tok0);  // position of the run's first token
+  const int q_end = q0 + a.queries < q_len ? q0 + a.queries : q_len;
+  const int32_t* table = a.tables + static_cast<size_t>(seq) * a.table_stride;
+
+  // what the workgroup reads: keys lo_min .. pos_max, in chunks of 64 from key_begin on
+  const int pos_min = start + q0, pos_max = start + q_end - 1;
+  const int lo_min = first_key(pos_min, a.window, a.block), lo_max = first_key(pos_max, a.window, a.block);
+  const int key_begin = lo_min & ~63;
+  const int nchunks = pos_max < 0 ? 0 : (pos_max - key_begin) / 64 + 1;
+  const int per_split = (nchunks + a.nsplit - 1) / a.nsplit;
+  const int c_first = z * per_split;
+  const int c_end = c_first + per_split < nchunks ? c_first + per_split : nchunks;
+
+  // the lane's row (both halves of the wavefront hold the same 32); a lane without one reads no key
+  const int row = wave * 32 + col, qi = q0 + row / group, head = kvh * group + row % group;
+  const bool mine = row < a.queries * group && qi < q_end;
+  const int q_pos = mine ? start + qi : -1, q_lo = first_key(q_pos, a.window, a.block);
+  bf16x8 qf[KS];
+  {
+    const bf16* src = a.q + static_cast<size_t>(tok0 + (mine ? qi : q0)) * a.q_stride + static_cast<size_t>(mine ? head : kvh * group) * D + half * 8;
+#pragma unroll
+    for (int st = 0; st < KS; ++st) qf[st] = *reinterpret_cast<const bf16x8*>(src + st * 16);
+  }
+  float m = -INFINITY, l = 0.f;  // the maximum of the unscaled scores; the lane's share of the sum
+  f32x16 o[DB];                  // element db * 32 + 8 g + 4 half + r of the row in register g * 4 + r
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+  const float scale2 = a.scale * 1.4426950408889634f;
+
+  // ---- what this thread brings of a chunk.  Piece x < kPieces: 16 codes of a key (block x / D; within it slab, key, half of the
+  // slab); the others: an element's codes of a block's 16 keys.  All lanes of a wavefront bring the same kind.
+  const size_t row_bytes = static_cast<size_t>(a.page_size) * D;
+  struct Held {
+    u32x4 codes;
+    u32x4 exps;  // of keys: the key's byte in the first word
+  };
+  auto piece = [&](int i) { return (wave * kWave + lane + i * kThreads) % (2 * kPieces); };
+  auto is_key = [&](int i) { return (wave * kWave + i * kThreads) % (2 * kPieces) < kPieces; };
+  auto fetch = [&](Held (&held)[kPer], int chunk) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int x = piece(i) % kPieces, y = x % D;
+      int key = key_begin + 64 * (chunk < nchunks ? chunk : nchunks - 1) + x / D * 16;
+      key = key > lo_min ? key : lo_min;  // a block that the sequence holds
+      key = key < pos_max ? key : pos_max;
+      if (D % 64 == 0) key = __builtin_amdgcn_readfirstlane(key);  // (a wavefront's pieces are of one block)
+      const int entry = pd.div(key), slot = (key - entry * a.page_size) & ~15;
+      const int page = table[entry < a.table_stride ? entry : a.table_stride - 1];
+      const size_t part = static_cast<size_t>(page >= 0 && page < a.num_pages ? page : 0) * a.kv_heads + kvh;  // (never outside the pool)
+      if (is_key(i)) {
+        const int of_block = y % 32 / 2;
+        held[i].codes = *reinterpret_cast<const u32x4*>(a.k_pool + part * row_bytes + static_cast<size_t>(y / 32) * a.page_size * 32 +
+                                                         (slot + of_block) * 32 + y % 2 * 16);
+        held[i].exps[0] = a.scales[part * 2 * a.page_size + slot + of_block];
+      } else {
+        held[i].codes = *reinterpret_cast<const u32x4*>(a.v_pool + part * row_bytes + static_cast<size_t>(y) * a.page_size + slot);
+        held[i].exps = *reinterpret_cast<const u32x4*>(a.scales + (part * 2 + 1) * a.page_size + slot);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto put = [&](const Held (&held)[kPer], int chunk, int buf) {
+    char* keys = reinterpret_cast<char*>(&mem[buf][0]);
+    char* values = keys + kSide;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int x = piece(i) % kPieces, y = x % D, blk = x / D;
+      const u32x4 w = held[i].codes;
+      if (is_key(i)) {
+        const int of_block = y % 32 / 2;
+        const float unit = __uint_as_float(held[i].exps[0] << 23);
+        char* at = keys + (blk * DB + y / 32) * 1024 + of_block * 64;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          *reinterpret_cast<bf16x8*>(at + ((y % 2 * 2 + p) ^ (of_block / 4)) * 16) = bf16_of_codes(w[2 * p], w[2 * p + 1], unit);
+      } else {
+        char* at = values + (blk * DB + y / 32) * 1024 + y % 32 * 32;
+        const int first = key_begin + 64 * chunk + blk * 16;
+        const bool edge = first < lo_min || first + 15 > pos_max;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          bf16x8 v;
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const int word = 2 * p + e / 4;
+            const auto pair = e % 4 ? __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[word]), true)
+                                    : __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[word]), false);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              float f = pair[b] * __uint_as_float((held[i].exps[word] >> ((e % 4 + b) * 8) & 0xffu) << 23);
+              // a slot that no query reads may hold anything, and its weight of 0 times that has to be 0
+              const int key = first + 8 * p + e + b;
+              if (edge && (key < lo_min || key > pos_max)) f = 0.f;
+              v[e + b] = static_cast<__bf16>(f);
+            }
+          }
+          *reinterpret_cast<bf16x8*>(at + (p ^ (y % 32 / 8 % 2)) * 16) = v;
+        }
+      }
+    }
+  };
+
+  // ---- where this lane's operands lie
+  const int key = 16 * (col / 16) + 8 * (col / 4 % 2) + 4 * (col / 8 % 2) + col % 4;  // of a tile's 32: its row `col`
+  const int turn = key % 16 / 4;
+  const int kat = key / 16 * DB * 1024 + key % 16 * 64, vat = kSide + col * 32 + (half ^ (col / 8 % 2)) * 16;
+
+  const int last_plain = (pos_min + 1 - key_begin) / 64 - 1;  // the last chunk that every query reads whole, and the first
+  const int first_plain = lo_max > key_begin ? (lo_max - key_begin + 63) / 64 : 0;
+  auto attend = [&](int buf, int chunk) {
+    const char* lds = reinterpret_cast<const char*>(&mem[buf][0]);
+    f32x16 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(lds + 2 * t * DB * 1024 + kat + st / 2 * 1024 + ((st % 2 * 2 + half) ^ turn) * 16);
+        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st], s[t], 0, 0, 0);
+      }
+    }
+    const int kb = key_begin + 64 * chunk;
+    if (chunk > last_plain || chunk < first_plain) {  // some query does not read all of it
+      asm volatile("");  // (stays a branch)
+      // register e of tile t is key 32 t + 16 (e / 8) + 8 half + e % 8
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int at = kb + 32 * t + e / 8 * 16 + 8 * half + e % 8;
+          if (at > q_pos || at < q_lo) s[t][e] = -INFINITY;
+        }
+    }
+    float mx = fmaxf(s[1][0], s[1][1]);
+#pragma unroll
+    for (int e = 2; e < 16; ++e) mx = fmaxf(mx, s[1][e]);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[0][e]);
+    {
+      const unsigned b = __builtin_bit_cast(unsigned, mx);
+      const auto halves = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+      mx = fmaxf(bits_as_float(halves[0]), bits_as_float(halves[1]));
+    }
+    const float m_new = fmaxf(m, mx);
+    const float m_safe = m_new == -INFINITY ? 0.f : m_new;  // (a row that has read no key yet)
+    const float alpha = __builtin_amdgcn_exp2f((m - m_safe) * scale2), shift = -m_safe * scale2;
+    m = m_new;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    bf16x8 p[4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[t][e], scale2, shift));
+        sum[e % 4] += w;
+        p[2 * t + e / 8][e % 8] = static_cast<__bf16>(w);
+      }
+    l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {  // some row's maximum rose
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] *= alpha;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const bf16x8 vf = *reinterpret_cast<const bf16x8*>(lds + vat + (u * DB + db) * 1024);
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, p[u], o[db], 0, 0, 0);
+      }
+  };
+
+  if (c_first < c_end) {  // the same for every wavefront of the workgroup
+    Held held[kPer];
+    fetch(held, c_first);
+    put(held, c_first, 0);
+    fetch(held, c_first + 1);
+    for (int c = c_first; c < c_end; ++c) {
+      const int buf = (c - c_first) % 2;
+      __syncthreads();  // chunk c is in LDS, and nobody reads chunk c - 1 any more
+      attend(buf, c);
+      put(held, c + 1, 1 - buf);  // (behind the last chunk: the last block again, which nobody reads)
+      fetch(held, c + 2);
+    }
+  }
+
+  float total = l;
+  {
+    const unsigned b = __builtin_bit_cast(unsigned, l);
+    const auto halves = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    total = bits_as_float(halves[0]) + bits_as_float(halves[1]);
+  }
+  if (!mine) return;
+  if (a.nsplit > 1) {
+    // a share's result, for merge_e4m3_kernel: O [row][share][D], then (maximum, sum) [row][share][2]
+    const size_t rows = static_cast<size_t>(a.n - a.first_seq) * a.heads;
+    const size_t at = static_cast<size_t>(tok0 + qi - a.first_seq) * a.heads + head;
+    float* dst = a.partial + (at * a.nsplit + z) * D + 4 * half;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(dst + db * 32 + g * 8) = f32x4{o[db][g * 4], o[db][g * 4 + 1], o[db][g * 4 + 2], o[db][g * 4 + 3]};
+    if (!half)
+      *reinterpret_cast<float2*>(a.partial + rows * a.nsplit * D + (at * a.nsplit + z) * 2) =
+          make_float2(m * scale2, total);
+    return;
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;  // (a query that reads no key: zeros)
+  bf16* dst = a.out + (static_cast<size_t>(tok0 + qi) * a.heads + head) * D + 4 * half;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      bf16x4 v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = static_cast<__bf16>(o[db][g * 4 + r] * inv);
+      *reinterpret_cast<bf16x4*>(dst + db * 32 + g * 8) = v;
+    }
+}
+
 }  // namespace shk
 
 using namespace shk;
@@ -107,5 +699,111 @@ extern "C" int shk_attention_e4m3(const void* q, int q_stride, void* out, int dt
                                                                  heads, positions, token_seq, tables, table_stride, num_seqs, pools,
                                                                  window, chunk, scale);
   SHK_LAUNCH_CHECK("attention_e4m3");
+  return 0;
+}
+
+namespace {
+
+// What every entry point on the matrix units asks for.
+int check_mfma(const char* who, int heads, int kv_heads, int head_dim, int page_size, int num_pages, int table_stride, int q_stride,
+               int nsplit, float scale) {
+  SHK_REQUIRE(shk_attention_e4m3_supports_mfma(heads, kv_heads, head_dim, page_size, q_stride),
+              "%s: not built for %d heads over %d of %d elements, pages of %d, rows %d apart", who, heads, kv_heads, head_dim, page_size,
+              q_stride);
+  SHK_REQUIRE(num_pages > 0 && table_stride > 0, "%s: bad cache sizes num_pages=%d table_stride=%d", who, num_pages, table_stride);
+  SHK_REQUIRE(nsplit >= 1 && nsplit <= kMaxShares, "%s: %d shares of the keys, 1..%d are built", who, nsplit, kMaxShares);
+  SHK_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive, got %g", who, scale);
+  return 0;
+}
+
+uint32_t page_magic(int page_size) { return static_cast<uint32_t>(((1ull << 32) + page_size - 1) / page_size); }
+
+template <int D>
+void merge_e4m3(int rows, hipStream_t s, const float* partial, void* out, int nsplit) {
+  merge_e4m3_kernel<D><<<rows, kWave, 0, s>>>(partial, static_cast<bf16*>(out), nsplit);
+}
+
+#define E4M3_BY_DIM(head_dim, CASE) \
+  switch (head_dim) {               \
+    case 32: CASE(32); break;       \
+    case 64: CASE(64); break;       \
+    case 96: CASE(96); break;       \
+    case 128: CASE(128); break;     \
+    case 160: CASE(160); break;     \
+    case 192: CASE(192); break;     \
+    case 224: CASE(224); break;     \
+    case 256: CASE(256); break;     \
+  }
+
+}  // namespace
+
+extern "C" int shk_attention_e4m3_supports_mfma(int heads, int kv_heads, int head_dim, int page_size, int q_stride) {
+  return heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 128 && head_dim >= 32 && head_dim <= 256 &&
+         head_dim % 32 == 0 && page_size > 0 && page_size % 16 == 0 && q_stride >= heads * head_dim && q_stride % 8 == 0;
+}
+
+extern "C" int shk_attention_decode_e4m3(const void* q, int q_stride, void* out, int num_seqs, int heads, int kv_heads, int head_dim,
+                                         const int32_t* positions, const int32_t* tables, int table_stride, int table_rows,
+                                         const void* k_pool, const void* v_pool, const void* scales, int page_size, int num_pages,
+                                         int window, int chunk, float scale, float* partial, int nsplit, void* stream) {
+  if (const int status = check_mfma("attention_decode_e4m3", heads, kv_heads, head_dim, page_size, num_pages, table_stride, q_stride,
+                                    nsplit, scale))
+    return status;
+  SHK_REQUIRE(num_seqs >= 0 && num_seqs <= 65535 && num_seqs <= table_rows, "attention_decode_e4m3: %d sequences, tables of %d",
+              num_seqs, table_rows);
+  if (num_seqs == 0) return 0;
+  SHK_REQUIRE(q && out && positions && tables && k_pool && v_pool && scales && (partial || nsplit == 1),
+              "attention_decode_e4m3: null pointer");
+  SHK_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0, "attention_decode_e4m3: rows of q must be 16-byte aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int head_tiles = (heads / kv_heads + 15) / 16;
+  const dim3 grid(kv_heads * head_tiles, num_seqs, nsplit);
+#define LAUNCH(D)                                                                                                                \
+  attention_decode_e4m3_kernel<D, 4><<<grid, 4 * kWave, 0, s>>>(                                                                 \
+      static_cast<const bf16*>(q), q_stride, static_cast<bf16*>(out), heads, head_tiles, positions, tables, table_stride,        \
+      static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(scales), kv_heads,   \
+      page_size, page_magic(page_size), num_pages, window, chunk, scale, partial, nsplit);                                       \
+  if (nsplit > 1) merge_e4m3<D>(num_seqs * heads, s, partial, out, nsplit)
+  E4M3_BY_DIM(head_dim, LAUNCH)
+#undef LAUNCH
+  SHK_LAUNCH_CHECK("attention_decode_e4m3");
+  return 0;
+}
+
+extern "C" int shk_attention_prefill_e4m3(const void* q, int q_stride, void* out, int n, int first_seq, int num_seqs, int heads,
+                                          int kv_heads, int head_dim, const int32_t* cu_q, const int32_t* ctx_lens,
+                                          const int32_t* tables, int table_stride, int table_rows, const void* k_pool,
+                                          const void* v_pool, const void* scales, int page_size, int num_pages, int window, int chunk,
+                                          float scale, float* partial, int nsplit, void* stream) {
+  if (const int status = check_mfma("attention_prefill_e4m3", heads, kv_heads, head_dim, page_size, num_pages, table_stride, q_stride,
+                                    nsplit, scale))
+    return status;
+  SHK_REQUIRE(first_seq >= 0 && num_seqs >= 0 && first_seq + num_seqs <= table_rows && n >= first_seq,
+              "attention_prefill_e4m3: sequences %d .. %d of %d rows, tables of %d", first_seq, first_seq + num_seqs, n, table_rows);
+  if (num_seqs == 0 || n == first_seq) return 0;
+  SHK_REQUIRE(q && out && cu_q && ctx_lens && tables && k_pool && v_pool && scales && (partial || nsplit == 1),
+              "attention_prefill_e4m3: null pointer");
+  SHK_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
+              "attention_prefill_e4m3: rows must be 16-byte aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int tokens = n - first_seq, group = heads / kv_heads;
+  auto groups = [&](int rows) { return static_cast<long long>(tokens / (rows / group) + num_seqs) * kv_heads * nsplit; };
+  const bool wide = head_dim <= 128 && groups(256) >= 256;
+  const long long count = groups(wide ? 256 : 128);
+  SHK_REQUIRE(count < (1LL << 31) && static_cast<long long>(tokens) * heads < (1LL << 31), "attention_prefill_e4m3: too many tokens: %d",
+              tokens);
+  const PortionArgs a{static_cast<const bf16*>(q), static_cast<bf16*>(out), cu_q, ctx_lens, tables, static_cast<const uint8_t*>(k_pool),
+                      static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(scales), partial, n, q_stride, heads, kv_heads,
+                      (wide ? 256 : 128) / group, first_seq, num_seqs, table_stride, page_size, num_pages, window, chunk, nsplit,
+                      page_magic(page_size), scale};
+#define LAUNCH(D)                                                                                                          \
+  if (wide)                                                                                                                \
+    attention_portion_e4m3_kernel<(D <= 128 ? D : 32), 8><<<static_cast<unsigned>(count), 8 * kWave, 0, s>>>(a);           \
+  else                                                                                                                     \
+    attention_portion_e4m3_kernel<D, 4><<<static_cast<unsigned>(count), 4 * kWave, 0, s>>>(a);                             \
+  if (nsplit > 1) merge_e4m3<D>(tokens * heads, s, partial, static_cast<bf16*>(out) + static_cast<size_t>(first_seq) * heads * D, nsplit)
+  E4M3_BY_DIM(head_dim, LAUNCH)
+#undef LAUNCH
+  SHK_LAUNCH_CHECK("attention_prefill_e4m3");
   return 0;
 }

@@ -80,6 +80,8 @@ const Launcher kLaunchers[] = {
     SHK_LAUNCHER(shk_rope_kv_store_e4m3),
     SHK_LAUNCHER(shk_kv_read_e4m3),
     SHK_LAUNCHER(shk_attention_e4m3),
+    SHK_LAUNCHER(shk_attention_decode_e4m3),
+    SHK_LAUNCHER(shk_attention_prefill_e4m3),
     SHK_LAUNCHER(shk_qkv_store),
     SHK_LAUNCHER(shk_latent_prepare),
     SHK_LAUNCHER(shk_rotate_heads),

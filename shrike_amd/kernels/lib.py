@@ -126,6 +126,10 @@ _SIGNATURES = {
                                _P, _I, _P],
     "shk_kv_read_e4m3": [_P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _P],
     "shk_attention_e4m3": [_P, _I, _P, _I, _I, _I, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _F, _P],
+    "shk_attention_e4m3_supports_mfma": [_I, _I, _I, _I, _I],
+    "shk_attention_decode_e4m3": [_P, _I, _P, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _F, _P, _I, _P],
+    "shk_attention_prefill_e4m3": [_P, _I, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _F, _P, _I,
+                                   _P],
     "shk_attention_supports_mfma": [_I, _I, _I, _I, _I],
     "shk_attention_decode_bf16": [_P, _I, _P, _I, _I, _I, _I, _P, _P, _I, _P, _P, _I, _I, _I, _F, _P, _I, _I, _I, _F, _P,
                                   _P, _I, _P],

@@ -903,6 +903,59 @@ def attention_e4m3(q, out, heads, kv_heads, head_dim, positions, token_seq, tabl
         int(chunk or 0), float(scale), _stream()))
 
 
+def attention_e4m3_supports_mfma(heads, kv_heads, head_dim, page_size, q_stride) -> bool:
+    """Whether attention_decode_e4m3 and attention_prefill_e4m3 take these sizes; attention_e4m3 takes all."""
+    return bool(load().shk_attention_e4m3_supports_mfma(heads, kv_heads, head_dim, page_size, q_stride))
+
+
+def _e4m3_rows(who, q, out, heads, head_dim, partial, rows, nsplit) -> int | None:
+    """Checks of the kernels on the matrix units; the scratch's address, None where there is one share."""
+    _rows(q, who + " q")
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+        raise KernelError(f"{who}: bfloat16 only")
+    if q.shape[1] < heads * head_dim or out.dim() != 2 or out.shape[1] != heads * head_dim or not out.is_contiguous():
+        raise KernelError(f"{who}: out must be contiguous rows of heads * head_dim, q at least as wide")
+    if nsplit <= 1:
+        return None
+    need = rows * heads * nsplit * (head_dim + 2)
+    if partial is None or partial.dtype != torch.float32 or not partial.is_contiguous() or partial.numel() < need:
+        raise KernelError(f"{who}: {nsplit} shares of {rows} rows' keys need a contiguous float32 scratch of {need} values")
+    return _dev(partial, "partial")
+
+
+def attention_decode_e4m3(q, out, num_seqs, heads, kv_heads, head_dim, positions, tables, k_pool, v_pool, scales, page_size, window, scale,
+                          partial=None, nsplit: int = 1, chunk=None) -> None:
+    """attention_decode() over a quantised cache: the first num_seqs rows of q, one token per sequence; nsplit workgroups share a
+    token's keys, through `partial` (float32, num_seqs * heads * nsplit * (head_dim + 2) values) where they are more than one."""
+    scratch = _e4m3_rows("attention_decode_e4m3", q, out, heads, head_dim, partial, num_seqs, nsplit)
+    if q.shape[0] < num_seqs or out.shape[0] < num_seqs:
+        raise KernelError("attention_decode_e4m3: fewer rows than sequences")
+    _step_rows("attention_decode_e4m3", num_seqs, positions)
+    check(load().shk_attention_decode_e4m3(
+        _dev(q, "q"), q.stride(0), _dev(out, "out"), num_seqs, heads, kv_heads, head_dim, _dev(positions, "positions", torch.int32),
+        *_e4m3_cache("attention_decode_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size), int(window or 0),
+        int(chunk or 0), float(scale), scratch, nsplit, _stream()))
+
+
+def attention_prefill_e4m3(q, out, first_seq, num_seqs, heads, kv_heads, head_dim, cu_q, ctx_lens, tables, k_pool, v_pool, scales,
+                           page_size, window, scale, partial=None, nsplit: int = 1, chunk=None) -> None:
+    """Causal attention of prompt portions over a quantised cache: rows first_seq .. of q and out, the new tokens of sequences first_seq ..
+    first_seq + num_seqs - 1 (sequences before have one token each, which are not touched): rows cu_q[s] .. cu_q[s + 1], the last of
+    ctx_lens[s] tokens.  nsplit workgroups share a run of queries' keys, through `partial` (float32, (rows of q - first_seq) * heads *
+    nsplit * (head_dim + 2) values) where they are more than one."""
+    n = q.shape[0]
+    scratch = _e4m3_rows("attention_prefill_e4m3", q, out, heads, head_dim, partial, n - first_seq, nsplit)
+    if out.shape[0] != n:
+        raise KernelError("attention_prefill_e4m3: out must have a row for each of q's")
+    _step_rows("attention_prefill_e4m3", first_seq + num_seqs, ctx_lens)
+    _step_rows("attention_prefill_e4m3", first_seq + num_seqs + 1, cu_q)
+    check(load().shk_attention_prefill_e4m3(
+        _dev(q, "q"), q.stride(0), _dev(out, "out"), n, first_seq, num_seqs, heads, kv_heads, head_dim, _dev(cu_q, "cu_q", torch.int32),
+        _dev(ctx_lens, "ctx_lens", torch.int32),
+        *_e4m3_cache("attention_prefill_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size), int(window or 0),
+        int(chunk or 0), float(scale), scratch, nsplit, _stream()))
+
+
 def qkv_store(qkv, heads, kv_heads, head_dim, v_dim, positions, token_seq, tables, k_pool, v_pool, page_size,
               q_temperature=None, v_norm_eps=None, write_kv=True, qk_norm_eps=None, q_weight=None, k_weight=None,
               has_kv=True) -> None:

@@ -149,6 +149,27 @@ def decode_streams(num_seqs: int, kv_heads: int, head_dim: int, max_ctx: int, wi
     return _pow2(num_seqs) * keys * kv_heads * head_dim * 4 >= STREAMING_FROM_BYTES
 
 
+def e4m3_decode_splits(num_seqs: int, heads: int, kv_heads: int, head_dim: int, max_ctx: int) -> int:
+    """Workgroups that share a single token's keys in a quantised cache: as many as put one on every compute unit, each with at
+    least KEYS_PER_WORKGROUP keys for its four wavefronts.  Rounded up as in decode_splits()."""
+    tiles = kv_heads * -(-heads // (16 * kv_heads))
+    want = -(-compute_units() // (_pow2(num_seqs) * tiles))
+    most = max(1, _pow2(max_ctx, KEYS_PER_WORKGROUP) // KEYS_PER_WORKGROUP)
+    return max(1, min(want, most, MAX_KEY_SPLITS))
+
+
+def e4m3_portion_splits(q_lens, starts, heads: int, kv_heads: int, head_dim: int, reach: int) -> int:
+    """Workgroups that share the keys of a run of queries in a quantised cache (`reach`: the most keys that a query reads): as many
+    as bring the launch to the number of compute units, each worth KEYS_PER_WORKGROUP keys or more on average."""
+    queries = max(1, 128 // (heads // kv_heads))
+    runs, keys, total = 0, 0, 0
+    for n, start in zip(q_lens, starts):
+        runs += -(-n // queries)
+        keys += n * min(start + n // 2, reach)
+        total += n
+    return max(1, min(compute_units() // max(1, runs * kv_heads), keys // max(1, total) // KEYS_PER_WORKGROUP, MAX_KEY_SPLITS))
+
+
 @dataclass
 class AttentionPlan:
     """How one step's attention is launched for a (heads, kv heads, head size)."""

@@ -115,6 +115,8 @@ def attention(step, q, keys, values, heads, scale, window=None, chunk=None):
     out, size, reach = torch.zeros_like(q), torch.zeros_like(q), torch.zeros(n, heads, 1, dtype=torch.float64)
     t = 0
     for i, (start, new) in enumerate(zip(step.starts, step.news)):
+        if new == 0:
+            continue
         k, v = step.rows(keys, i, start + new), step.rows(values, i, start + new)
         for h in range(heads):
             g = h * kv // heads
