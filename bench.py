@@ -323,7 +323,8 @@ TIMED_OPS = ("embed", "add_rmsnorm", "act_mul", "gemm", "gemm_f32_tiled_weight",
              "xielu", "add_layernorm", "attention_talking", "attention_talking_mfma", "short_conv", "dt_softplus", "selective_scan",
              "rotate_half_rows", "retention_scan", "retention_chunk", "moe_route", "moe_experts", "moe_few", "mix_history",
              "scale_softcap", "postnorm", "cast_rows", "activate", "gate_mul", "add_dynamic_tanh", "conv_store", "diff_attention",
-             "diff_attention_decode", "diff_attention_prefill", "rglru", "gla_chunk")
+             "diff_attention_decode", "diff_attention_prefill", "rglru", "gla_chunk", "rope_kv_store_e4m3", "kv_read_e4m3",
+             "attention_e4m3", "attention_decode_e4m3", "attention_prefill_e4m3")
 
 
 def timed_label(name: str, args, kwargs) -> str:

@@ -35,6 +35,8 @@ def parse_args(argv=None) -> argparse.Namespace:
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--no-chat", action="store_true", help="do not wrap a text prompt in the chat template")
     ap.add_argument("--dtype", choices=["bfloat16", "float32", "bf16", "fp32"], default=None)
+    ap.add_argument("--cache-dtype", choices=["auto", "e4m3", "fp8"], default="auto",
+                    help="how keys and values are kept: in the compute dtype (auto) or as 8-bit codes")
     ap.add_argument("--block-size", type=int, default=16)
     ap.add_argument("--num-kv-blocks", type=int, default=None)
     ap.add_argument("--gpu-mem-util", type=float, default=0.85)
@@ -57,7 +59,7 @@ def main(argv=None) -> int:
         block_size=args.block_size, gpu_mem_util=args.gpu_mem_util,
         max_tokens_per_step=args.max_tokens_per_step, max_running=args.max_running,
         enable_prefix_caching=not args.no_prefix_caching, num_kv_blocks=args.num_kv_blocks,
-        dtype=args.dtype, seed=args.seed, graphs=not args.no_graphs, overlap_steps=not args.no_overlap,
+        dtype=args.dtype, cache_dtype=args.cache_dtype, seed=args.seed, graphs=not args.no_graphs, overlap_steps=not args.no_overlap,
     )
     if args.random_config is not None:
         import json
@@ -83,8 +85,9 @@ def main(argv=None) -> int:
         arch = get_architecture(architecture_name(raw))
         spec = arch.build_spec(arch.config_cls.from_dict(raw))
         dtype = canonical_dtype(args.dtype) if args.dtype else spec.stored_dtype
-        model, runtime = random_model(spec, seed=args.seed, dtype=dtype)
-        engine = LLMEngine(None, EngineConfig(**dict(options, dtype=dtype)), model=model, runtime=runtime)
+        config = EngineConfig(**dict(options, dtype=dtype))
+        model, runtime = random_model(spec, seed=args.seed, dtype=dtype, cache_dtype=config.cache_dtype)
+        engine = LLMEngine(None, config, model=model, runtime=runtime)
     else:
         engine = LLMEngine(args.model, **options)
     print(f"[engine up in {time.perf_counter() - t0:.1f}s, {engine.cache.num_pages} KV blocks]",

@@ -15,6 +15,19 @@ def canonical_dtype(name: str) -> str:
         raise ValueError(f"dtype must be bfloat16 or float32, got {name!r}") from None
 
 
+_CACHE_DTYPES = {"e4m3": "e4m3", "fp8": "e4m3", "fp8_e4m3": "e4m3", "float8_e4m3fn": "e4m3"}
+
+
+def canonical_cache_dtype(name: str | None) -> str | None:
+    """"e4m3", or None for a cache in the compute dtype."""
+    if name is None or name == "auto":
+        return None
+    try:
+        return _CACHE_DTYPES[str(name).replace("torch.", "")]
+    except KeyError:
+        raise ValueError(f"cache_dtype must be None (the compute dtype) or e4m3, got {name!r}") from None
+
+
 @dataclass
 class EngineConfig:
     """block_size, gpu_mem_util, max_tokens_per_step, max_running and
@@ -24,6 +37,10 @@ class EngineConfig:
         device memory times gpu_mem_util (shrike/engine/model_runner.py:165-174).
     dtype: "bfloat16" (serving kernels) or "float32" (every kernel in true
         32-bit arithmetic); None takes the dtype the model folder was stored in.
+    cache_dtype: None keeps keys and values in the compute dtype; "e4m3" (or "fp8") as 8-bit codes
+        with a power of two per token and head: half the bytes of bfloat16 and twice the tokens in
+        the same memory, for models whose every layer is attention that rotates its keys or
+        stores them as they are (others are refused).
     graphs: replay decode-only steps from HIP graphs.
     overlap_steps: launch the next decode step before the host has read the
         tokens of this one (they pass from the sampler to the next step on the
@@ -38,6 +55,7 @@ class EngineConfig:
     enable_prefix_caching: bool = True
     num_kv_blocks: int | None = None
     dtype: str | None = None
+    cache_dtype: str | None = None
     seed: int = 0
     graphs: bool = True
     overlap_steps: bool = True
@@ -56,3 +74,4 @@ class EngineConfig:
             raise ValueError(f"num_kv_blocks must be >= 1, got {self.num_kv_blocks}")
         if self.dtype is not None:
             self.dtype = canonical_dtype(self.dtype)
+        self.cache_dtype = canonical_cache_dtype(self.cache_dtype)

@@ -9,7 +9,7 @@ this level knows which architecture it came from.
 
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import ClassVar
 
 # Every part finds its tensors under its own name plus a sub-name per role ("weight",
@@ -108,7 +108,9 @@ class AttentionSpec:
     their norms' weights); it reads the cache of another run (ScheduleEntry.cache_of) with its
     own queries and mask.  ``cache_window``: what the layer's cache keeps where that is not its
     own window, because a run that reads this cache looks further back ("own": the window;
-    None: everything).
+    None: everything).  ``cache_dtype``: None keeps keys and values in the compute dtype; "e4m3" keeps
+    them as 8-bit codes with a power of two per token and key/value head (csrc/e4m3.h); built for the attention that rotates or
+    stores its keys as they are: without values of another size, temperatures, norms, caps, sinks, biases and mixed heads.
     """
 
     kind: ClassVar[str] = "paged_attention"
@@ -135,6 +137,7 @@ class AttentionSpec:
     bucket_bias: tuple | None = None
     shared_kv: bool = False
     cache_window: object = "own"
+    cache_dtype: str | None = None
 
 
 @dataclass(frozen=True)
@@ -637,3 +640,18 @@ class ModelSpec:
                         f"schedule[{pos}] reads the cache of position {entry.cache_of}, "
                         "which does not own one"
                     )
+
+
+def with_cache_dtype(spec: ModelSpec, cache_dtype: str | None) -> ModelSpec:
+    """The model with keys and values kept as `cache_dtype` says (AttentionSpec.cache_dtype) in every layer; refused for a
+    model with another mixer that keeps something per page or with attention that a quantised cache is not built for."""
+    if cache_dtype is None:
+        return spec
+    blocks = []
+    for block in spec.blocks:
+        mixer = getattr(block, "mixer", None)
+        if type(mixer) is not AttentionSpec:
+            raise ValueError(f"{spec.architecture}: a cache in {cache_dtype} is built for paged attention, and {block.name} mixes by "
+                             f"{getattr(mixer, 'kind', type(mixer).__name__)}")
+        blocks.append(replace(block, mixer=replace(mixer, cache_dtype=cache_dtype)))
+    return replace(spec, blocks=tuple(blocks))

@@ -39,7 +39,7 @@ class EngineStats:
 class LLMEngine:
     """LLMEngine(model_dir, block_size=16, gpu_mem_util=0.85,
     max_tokens_per_step=512, max_running=256, enable_prefix_caching=True,
-    num_kv_blocks=None, dtype=None, seed=0)."""
+    num_kv_blocks=None, dtype=None, cache_dtype=None, seed=0)."""
 
     def __init__(self, model_dir: str, config: EngineConfig | None = None, *, model=None,
                  runtime=None, **options) -> None:
@@ -47,7 +47,10 @@ class LLMEngine:
         cfg = self.config
         self.model_dir = model_dir
         if model is None:
-            model, runtime, _ = load_model(model_dir, cfg.dtype, cfg.device)
+            model, runtime, _ = load_model(model_dir, cfg.dtype, cfg.device, cfg.cache_dtype)
+        elif cfg.cache_dtype is not None and any(getattr(b.mixer, "cache_dtype", None) != cfg.cache_dtype for b in model.spec.blocks):
+            raise ValueError(f"the model was built without a cache in {cfg.cache_dtype}: build it with "
+                             f"cache_dtype={cfg.cache_dtype!r} (load_model, random_model)")
         self.model, self.runtime = model, runtime
         self.tokenizer = _load_tokenizer(model_dir) if model_dir is not None else None
 

@@ -31,7 +31,8 @@ def compute_units() -> int:
 
 
 def kv_cache_spec(num_kv_heads: int, head_dim: int, window: int | None = None,
-                  chunk: int | None = None, value_dim: int | None = None, keep_first: int = 0) -> PagedSpec:
+                  chunk: int | None = None, value_dim: int | None = None, keep_first: int = 0,
+                  cache_dtype: str | None = None) -> PagedSpec:
     """The cache of grouped-query attention, laid out for this file's kernels: per
     page and key/value head the keys in slabs of 32 elements, [head_dim / 32,
     page_size, 32] (a wavefront's operand load for the matrix instruction then
@@ -39,11 +40,15 @@ def kv_cache_spec(num_kv_heads: int, head_dim: int, window: int | None = None,
     slab of head_dim elements where head_dim is no multiple of 32), and the values
     transposed, [head_dim, page_size] (the keys of a page side by side for every
     element, which is the operand layout of V^T).  `value_dim`: the size of a value
-    where it is not the keys' size."""
+    where it is not the keys' size.  `cache_dtype` "e4m3": the same layouts in 8-bit codes, and the
+    biased exponents of a power of two per token and head, the keys' before the values'."""
     slab = ops.key_slab(head_dim)
+    held, scales = None, ()
+    if cache_dtype is not None:
+        held, scales = "float8_e4m3fn", (PageTensor("scales", (num_kv_heads, 2, PAGE), "uint8"),)
     return PagedSpec(
-        tensors=(PageTensor("k", (num_kv_heads, head_dim // slab, PAGE, slab)),
-                 PageTensor("v", (num_kv_heads, head_dim if value_dim is None else value_dim, PAGE))),
+        tensors=(PageTensor("k", (num_kv_heads, head_dim // slab, PAGE, slab), held),
+                 PageTensor("v", (num_kv_heads, head_dim if value_dim is None else value_dim, PAGE), held), *scales),
         window=window,
         chunk=chunk,
         keep_first=keep_first,
@@ -343,6 +348,11 @@ class PagedAttention(Mixer):
                     or getattr(s, "bucket_bias", None) or self.shared_kv)
 
     @property
+    def cache_dtype(self) -> str | None:
+        """None: keys and values are kept in the compute dtype; "e4m3": as 8-bit codes."""
+        return getattr(self.spec, "cache_dtype", None)
+
+    @property
     def shared_kv(self) -> bool:
         """Whether the layer has no keys and values of its own and reads another run's cache."""
         return bool(getattr(self.spec, "shared_kv", False))
@@ -401,10 +411,15 @@ class PagedAttention(Mixer):
         s = self.spec
         kept = getattr(s, "cache_window", "own")
         return kv_cache_spec(s.num_kv_heads, s.head_dim, s.window if kept == "own" else kept, s.chunk,
-                             None if self.value_dim == s.head_dim else self.value_dim)
+                             None if self.value_dim == s.head_dim else self.value_dim, cache_dtype=self.cache_dtype)
 
     def check(self, runtime):
         s = self.spec
+        if self.cache_dtype not in (None, "e4m3"):
+            raise ValueError(f"{self.name}: cache_dtype must be None or e4m3, got {self.cache_dtype!r}")
+        if self.cache_dtype and (self.plain_store or not s.scale > 0):
+            raise ValueError(f"{self.name}: a cache in {self.cache_dtype} is built for attention that rotates its keys or stores them as "
+                             "they are, with values of their size and a positive scale")
         if self.plain_store:
             if self.position is not None or s.values_from_keys or s.qkv_bias:
                 raise ValueError(f"{self.name}: values of another size than keys, a query temperature, normed "
@@ -485,11 +500,11 @@ class PagedAttention(Mixer):
         s = self.spec
         return ("paged_attention", s.num_heads, s.num_kv_heads, s.head_dim, s.window, s.chunk, self.plain_store,
                 self.talking, self.value_dim, self._qkv_width(), bool(getattr(s, "bucket_bias", None)),
-                bool(getattr(s, "softcap", None)), bool(getattr(s, "sinks", False)))
+                bool(getattr(s, "softcap", None)), bool(getattr(s, "sinks", False)), bool(self.cache_dtype))
 
     def context_scratch_bytes(self, rows: int, keys: int) -> int:
         s = self.spec
-        if self.dtype != torch.float32 or self.talking:
+        if self.dtype != torch.float32 or self.talking or self.cache_dtype:
             return 0
         return 4 * f32_split_floats(rows, s.num_heads, s.num_kv_heads, self.value_dim, keys)
 
@@ -503,6 +518,19 @@ class PagedAttention(Mixer):
         s = self.spec
         h, hkv, d = s.num_heads, s.num_kv_heads, s.head_dim
         plan = shape.notes[key] = AttentionPlan()
+        if self.cache_dtype:
+            # the portions' kernel finds its workgroups' queries itself: no lists
+            plan.mfma = self.dtype == torch.bfloat16 and ops.attention_e4m3_supports_mfma(h, hkv, d, shape.page_size, self._qkv_width())
+            if plan.mfma:
+                reach = min(x for x in (s.window, s.chunk, 1 << 40) if x)
+                if shape.num_decode:
+                    plan.nsplit = e4m3_decode_splits(shape.num_decode, h, hkv, d, min(shape.max_decode_ctx, reach))
+                if shape.num_seqs > shape.num_decode:
+                    plan.portion_splits = e4m3_portion_splits(shape.q_lens[shape.num_decode:].tolist(),
+                                                              shape.starts[shape.num_decode:].tolist(), h, hkv, d, reach)
+                plan.first_token, plan.count = shape.num_decode, shape.num_seqs - shape.num_decode
+            shape.launch_key.append((key, plan.mfma, plan.nsplit, plan.portion_splits, plan.first_token, plan.count))
+            return
         if self.talking and self.dtype == torch.bfloat16 and ops.attention_talking_supports_mfma(
                 d, self.value_dim, shape.page_size, self._qkv_width()):
             # on the matrix units: single tokens by key/value head, prompt portions in tiles of 16 queries
@@ -590,6 +618,22 @@ class PagedAttention(Mixer):
             raise RuntimeError(f"{self.name}: the step was not prepared for this mixer "
                                "(the step function calls prepare() on every part)")
         q = qkv[:, : h * d]
+        if self.cache_dtype:
+            pages = (tables, cache.pools["k"], cache.pools["v"], cache.pools["scales"], cache.page_size, s.window, s.scale)
+            if not plan.mfma:
+                ops.attention_e4m3(q, out, h, hkv, d, ctx.positions, ctx.token_seq, *pages, chunk=s.chunk)
+                return
+            if ctx.num_decode:
+                partial = ctx.buffer("attn_partial", (ctx.num_decode * h * plan.nsplit * (d + 2),), torch.float32) \
+                    if plan.nsplit > 1 else None
+                ops.attention_decode_e4m3(q, out, ctx.num_decode, h, hkv, d, ctx.positions, *pages, partial, plan.nsplit, chunk=s.chunk)
+            if plan.count:
+                partial = ctx.buffer("attn_portion_partial",
+                                     ((ctx.num_tokens - plan.first_token) * h * plan.portion_splits * (d + 2),), torch.float32) \
+                    if plan.portion_splits > 1 else None
+                ops.attention_prefill_e4m3(q, out, plan.first_token, plan.count, h, hkv, d, ctx.cu_q, ctx.ctx_lens, *pages, partial,
+                                           plan.portion_splits, chunk=s.chunk)
+            return
         if plan.kernel == "talking_mfma":
             floats = ops.attention_talking_mfma_scratch_floats(q.shape[0], h, hkv, self.value_dim, ctx.num_decode,
                                                                plan.nsplit)
@@ -666,7 +710,7 @@ class PagedAttention(Mixer):
         """Whether the step's projections, their rotation and the cache write are one kernel (ops.few_heads).  It leaves the
         queries alone beside the cache, so not for an attend() of another class, which may read the step's keys and values too."""
         s = self.spec
-        if not self.ends_onto or type(self).attend is not PagedAttention.attend or self.plain_store or s.values_from_keys or self.position is None or getattr(self.position, "adjacent_pairs", False):
+        if not self.ends_onto or type(self).attend is not PagedAttention.attend or self.cache_dtype or self.plain_store or s.values_from_keys or self.position is None or getattr(self.position, "adjacent_pairs", False):
             return False
         table = self.position.rotary_table()
         return (table is not None and table[1] == s.head_dim and s.head_dim % 16 == 0 and self.w_qkv.tiled is not None
@@ -716,9 +760,10 @@ class PagedAttention(Mixer):
             self.linear(x, self.w_qkv, qkv, bias=self.b_qkv)
             self.position.apply(ctx, qkv, s.num_heads, s.num_kv_heads, s.head_dim)
         inv_freq, rot_dim = table if table is not None else (None, 0)
-        ops.rope_kv_store(
+        store, scales = (ops.rope_kv_store_e4m3, (cache.pools["scales"],)) if self.cache_dtype else (ops.rope_kv_store, ())
+        store(
             qkv, s.num_heads, s.num_kv_heads, s.head_dim, rot_dim, inv_freq, ctx.positions,
-            ctx.token_seq, tables, cache.pools["k"], cache.pools["v"], cache.page_size,
+            ctx.token_seq, tables, cache.pools["k"], cache.pools["v"], *scales, cache.page_size,
             write_kv=cache.owned, split_sum=split_sum,
             adjacent_pairs=bool(table is not None and getattr(self.position, "adjacent_pairs", False)),
             values_from_keys=s.values_from_keys,

@@ -233,12 +233,13 @@ def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="python -m shrike_amd.repl", description=__doc__.split("\n\n")[0])
     ap.add_argument("--model", default=DEFAULT_MODEL_DIR)
     ap.add_argument("--dtype", default=None)
+    ap.add_argument("--cache-dtype", choices=["auto", "e4m3", "fp8"], default="auto")
     ap.add_argument("--num-kv-blocks", type=int, default=None)
     args = ap.parse_args(argv)
     from .engine.llm_engine import LLMEngine
 
     t0 = time.perf_counter()
-    engine = LLMEngine(args.model, dtype=args.dtype, num_kv_blocks=args.num_kv_blocks)
+    engine = LLMEngine(args.model, dtype=args.dtype, cache_dtype=args.cache_dtype, num_kv_blocks=args.num_kv_blocks)
     print(f"{args.model}: {engine.cache.num_pages} cache pages, up in {time.perf_counter() - t0:.1f} s; "
           "/help lists the commands")
     Session(engine, args.model).run(_prompted_lines("shrike> "))

@@ -33,6 +33,8 @@ def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="trace_run", description=__doc__.split("\n\n")[0])
     ap.add_argument("--model", required=True, help="folder with config.json and model.safetensors")
     ap.add_argument("--dtype", required=True, choices=["bfloat16", "float32"])
+    ap.add_argument("--cache-dtype", choices=["auto", "e4m3", "fp8"], default="auto",
+                    help="how keys and values are kept: in the compute dtype (auto) or as 8-bit codes")
     ap.add_argument("--out", required=True, help="folder for <step>.f32 files")
     ap.add_argument("--max-tokens", type=int, required=True,
                     help="most tokens live requests hold at any time (each rounded up to 64)")
@@ -56,12 +58,13 @@ def main(argv=None) -> int:
     import torch
 
     from ..cache import CacheManager
+    from ..config.engine_config import canonical_cache_dtype
     from ..engine.loading import load_model
     from ..engine.runner import ModelRunner, StepEntry
     from .poison import PagePoisoner
 
     _say(f"loading {args.model} as {args.dtype}")
-    model, runtime, _cfg = load_model(args.model, args.dtype)
+    model, runtime, _cfg = load_model(args.model, args.dtype, cache_dtype=canonical_cache_dtype(args.cache_dtype))
     page = args.block_size
     num_pages = max(1, -(-args.max_tokens // page))
     cache = CacheManager(model.cache_specs(), page, num_pages, max_slots=args.max_requests,

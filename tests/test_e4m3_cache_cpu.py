@@ -65,3 +65,69 @@ def test_refusals_before_any_launch(lib):
                        (attend(ps=0), "page_size=0"), (attend(scale=0.0), "positive"), (attend(scale=float("nan")), "positive"),
                        (attend(n=70000), "65535"), (attend(), "null pointer")):
         refused(lib, name, args, part)
+
+
+def test_names_of_the_cache_dtype():
+    from shrike_amd.config import EngineConfig, canonical_cache_dtype
+
+    assert EngineConfig().cache_dtype is None and EngineConfig(cache_dtype="auto").cache_dtype is None
+    assert {canonical_cache_dtype(n) for n in ("e4m3", "fp8", "fp8_e4m3", "float8_e4m3fn", torch.float8_e4m3fn)} == {"e4m3"}
+    with pytest.raises(ValueError, match="e5m2"):
+        EngineConfig(cache_dtype="e5m2")
+
+
+def test_models_that_a_quantised_cache_is_not_built_for_are_refused():
+    from dataclasses import replace
+
+    from shrike_amd.config import architecture_name, get_architecture
+    from shrike_amd.config.specs import with_cache_dtype
+    from shrike_amd.models import DecoderModel
+
+    from .tiny import CONFIGS
+    from .tiny_bevovik import CONFIGS as BEVOVIK
+    from .tiny_fozedra import CONFIGS as FOZEDRA
+    from .tiny_minilorn import CONFIGS as MINILORN
+    from .tiny_mofarax import CONFIGS as MOFARAX
+
+    def spec_of(raw):
+        arch = get_architecture(architecture_name(raw))
+        return arch.build_spec(arch.config_cls.from_dict(raw))
+
+    for raw in (*CONFIGS.values(), *MOFARAX.values()):
+        spec = with_cache_dtype(spec_of(raw), "e4m3")
+        model = DecoderModel(spec)
+        for need in model.cache_specs():
+            assert [t.dtype for t in need.tensors] == ["float8_e4m3fn", "float8_e4m3fn", "uint8"]
+        for block in model.blocks:
+            block.mixer.check(None)
+        assert with_cache_dtype(spec_of(raw), None) == spec_of(raw)
+    for raw in (*BEVOVIK.values(), *FOZEDRA.values(), *MINILORN.values()):
+        spec = spec_of(raw)
+        try:
+            model = DecoderModel(with_cache_dtype(spec, "e4m3"))
+        except ValueError as e:
+            assert "is built for paged attention" in str(e)
+            continue
+        with pytest.raises(ValueError, match="is built for attention that rotates"):
+            for block in model.blocks:
+                block.mixer.check(None)
+    first = spec_of(CONFIGS["A"]).blocks[0].mixer
+    from shrike_amd.parts.attention import PagedAttention
+
+    with pytest.raises(ValueError, match="must be None or e4m3"):
+        PagedAttention(replace(first, cache_dtype="int4"), 64, "x").check(None)
+
+
+@pytest.mark.parametrize("heads, kv", [(14, 2), (28, 4), (16, 16), (40, 1), (128, 1)])
+def test_launch_plans(heads, kv):
+    from shrike_amd.parts.attention import e4m3_decode_splits, e4m3_portion_splits
+
+    for seqs in (1, 2, 7, 64, 300):
+        for ctx in (1, 63, 256, 257, 5000, 131072):
+            n = e4m3_decode_splits(seqs, heads, kv, 128, ctx)
+            assert 1 <= n <= 64
+            # a batch that is padded to the next power of two, and a longer context up to the next one, take the same
+            assert n == e4m3_decode_splits(1 << (seqs - 1).bit_length(), heads, kv, 128, max(256, 1 << (ctx - 1).bit_length()))
+    for lens, starts in (([2], [0]), ([512], [16000]), ([17] * 4, [700, 800, 900, 1900]), ([2048], [0]), ([1, 0, 30], [5, 0, 9])):
+        assert 1 <= e4m3_portion_splits(lens, starts, heads, kv, 128, 1 << 40) <= 64
+        assert e4m3_portion_splits(lens, starts, heads, kv, 128, 100) == 1  # a window of 100 keys is not shared
