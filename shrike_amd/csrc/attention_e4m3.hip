@@ -14,6 +14,7 @@ namespace shk {
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxShares = 64;  // workgroups that share a query's keys: a lane of the kernel that joins them each
@@ -377,12 +378,18 @@ __global__ void __launch_bounds__(kWave) merge_e4m3_kernel(const float* __restri
 
 // ------------------------------------------------------------------ portions
 // Runs of new tokens over the pages that hold what came before and the run itself.  A row is one query of one head; the heads that
-// share a key/value head read the same keys, so a workgroup takes all of them for a run of queries: 32 rows a wavefront, whatever
-// the heads of a group.  Products as above with v_mfma_f32_32x32x16_bf16: a lane owns half of a row's scores, and the weights go
-// from one product into the next without leaving it.
+// share a key/value head read the same keys, so a workgroup takes all of them for a run of queries: 128 rows, 32 a wavefront,
+// whatever the heads of a group.  Products as above with v_mfma_f32_32x32x16_bf16: a lane owns half of a row's scores, and the
+// weights go from one product into the next without leaving it.
 //
-// Chunks of 64 keys.  Codes come from the pages into registers a chunk ahead and go to LDS as bfloat16 values, each of them
-// converted once for all rows of the workgroup:
+// Two teams of four wavefronts (TEAMS = 2) share the rows and take the chunks of 64 keys by turns.  Each SIMD unit holds a wavefront
+// of either team, and barriers keep them half a turn apart: while one multiplies (the chunk before's weights with its values, this
+// chunk's scores), the other one does what the vector units have to: softmax arithmetic, and converting the next chunk.  Without
+// that both would want the same unit at the same time.  Their results are joined through LDS in the end.
+//
+// Codes come from the pages into registers a turn ahead and go to LDS as bfloat16 values, each of them converted once for the
+// team's rows; a wavefront brings one block of 16 keys of every chunk.  Keys get their power of two in the conversion; that of a value
+// joins its key's weight in float32, behind the sum of the weights and before they are rounded.
 //   keys    [block of 16][32 elements] units of 1 KiB, 64 bytes a key: piece c of 16 bytes of a key at place c ^ (key / 4),
 //   values  [block of 16][32 elements] units, 32 bytes an element: piece c at place c ^ (element / 8 % 2),
 // so that the lanes that LDS serves together meet no bank conflicts.  Row 8 a + 4 h + r of a score tile is key 16 (a / 2) + 8 h +
@@ -390,6 +397,9 @@ __global__ void __launch_bounds__(kWave) merge_e4m3_kernel(const float* __restri
 //
 // The workgroups find their queries themselves, a sequence's last queries (which read the most keys) first, so a step needs no
 // lists from the host.
+constexpr int kPortionRows = 128;
+constexpr float kLargeSum = 1024.f;  // of a chunk's weights relative to the reference: it moves
+
 struct PortionArgs {
   const bf16* q;
   bf16* out;
@@ -401,16 +411,20 @@ struct PortionArgs {
   float scale;
 };
 
-template <int D, int WAVES>
-__global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attention_portion_e4m3_kernel(PortionArgs a) {
+template <int D, int TEAMS, int PAGE>
+__global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4m3_kernel(PortionArgs a) {
   constexpr int KS = D / 16, DB = D / 32;
-  constexpr int kThreads = WAVES * kWave, kSide = 64 * D * 2;  // bytes of a chunk's keys as bfloat16
-  constexpr int kPieces = 4 * D;                               // of 16 codes of its keys (as many of its values)
-  constexpr int kPer = (2 * kPieces + kThreads - 1) / kThreads;
-  __shared__ u32x4 mem[2][2 * kSide / 16];
+  constexpr int kSide = 64 * D * 2;         // bytes of a chunk's keys as bfloat16, and of its values
+  constexpr int kPer = (D + kWave - 1) / kWave;  // pieces of 16 codes of a block's keys that a lane brings, and of its values
+  // a team's keys of two chunks and values of two; in the end the second team's results
+  __shared__ u32x4 mem[TEAMS][4 * kSide / 16];
+  __shared__ float units[TEAMS][2][64], ends[TEAMS][2][kPortionRows];  // (units: of the values)
+  static_assert(TEAMS == 1 || TEAMS * 4 * kSide >= kPortionRows * D * 4, "the second team's sums fit");
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int team = wave / 4, member = wave % 4;
   const int col = lane % 32, half = lane / 32;
-  const PageDiv pd{a.page_size, a.page_magic};
+  const int page_size = PAGE ? PAGE : a.page_size;
+  const PageDiv pd{page_size, a.page_magic};
   const int z = blockIdx.x % a.nsplit, kvh = blockIdx.x / a.nsplit % a.kv_heads;
 
   // ---- this workgroup's sequence and first query
@@ -441,9 +455,9 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attention_port
     q0 = __builtin_amdgcn_readfirstlane(q0);
   }
   const int group = a.heads / a.kv_heads;
-  const int tok0 = a.cu_q[seq], q_len = min(a.cu_q[seq + 1], a.n) - tok0;
+  const int tok0 = a.cu_q[seq], tok1 = a.cu_q[seq + 1], q_len = min(tok1, a.n) - tok0;
   if (tok0 < a.first_seq || q0 >= q_len) return;  // (ranges that are not the rows' are a mistake of the caller's, never followed)
-  const int start = a.ctx_lens[seq] - (a.cu_q[seq + 1] - tok0);  // position of the run's first token
+  const int start = a.ctx_lens[seq] - (tok1 - tok0);  // position of the run's first token
   const int q_end = q0 + a.queries < q_len ? q0 + a.queries : q_len;
   const int32_t* table = a.tables + static_cast<size_t>(seq) * a.table_stride;
 
@@ -456,8 +470,8 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attention_port
   const int c_first = z * per_split;
   const int c_end = c_first + per_split < nchunks ? c_first + per_split : nchunks;
 
-  // the lane's row (both halves of the wavefront hold the same 32); a lane without one reads no key
-  const int row = wave * 32 + col, qi = q0 + row / group, head = kvh * group + row % group;
+  // the lane's row (both halves of the wavefront hold the same 32, both teams all of them); a lane without one reads no key
+  const int row = member * 32 + col, qi = q0 + row / group, head = kvh * group + row % group;
   const bool mine = row < a.queries * group && qi < q_end;
   const int q_pos = mine ? start + qi : -1, q_lo = first_key(q_pos, a.window, a.block);
   bf16x8 qf[KS];
@@ -466,107 +480,202 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attention_port
 #pragma unroll
     for (int st = 0; st < KS; ++st) qf[st] = *reinterpret_cast<const bf16x8*>(src + st * 16);
   }
-  float m = -INFINITY, l = 0.f;  // the maximum of the unscaled scores; the lane's share of the sum
+  float m = -INFINITY, l = 0.f;  // the weights' reference, of the unscaled scores; the lane's share of the sum
   f32x16 o[DB];                  // element db * 32 + 8 g + 4 half + r of the row in register g * 4 + r
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
   const float scale2 = a.scale * 1.4426950408889634f;
+  float shift = 0.f, limit = mine ? -1.f : kLargeSum;  // what the scaled scores get; the sum from which on the reference moves
 
-  // ---- what this thread brings of a chunk.  Piece x < kPieces: 16 codes of a key (block x / D; within it slab, key, half of the
-  // slab); the others: an element's codes of a block's 16 keys.  All lanes of a wavefront bring the same kind.
-  const size_t row_bytes = static_cast<size_t>(a.page_size) * D;
-  struct Held {
-    u32x4 codes;
-    u32x4 exps;  // of keys: the key's byte in the first word
+  // ---- what this lane brings of its wavefront's block of a chunk: pieces y = lane, lane + 64, ... < D (some twice where D is no
+  // multiple of 64) of the keys (slab, key, half of the slab) and of the values (an element's codes of the 16 keys)
+  const int block_key = lane % 32 / 2;  // the key of the pieces, whatever y
+  uint32_t more_k[kPer], more_v[kPer], k_at[kPer], v_at[kPer];  // (more_: from where the first piece lies)
+  const uint32_t row_bytes = static_cast<uint32_t>(page_size) * D;
+  const uint8_t* my_keys = a.k_pool + lane / 32 * page_size * 32 + block_key * 32 + lane % 2 * 16;
+  const uint8_t* my_values = a.v_pool + lane % D * page_size;
+  if (D == 32) my_keys = a.k_pool + block_key * 32 + lane % 2 * 16;
+  const uint8_t* my_key_exps = a.scales + block_key;
+  const uint8_t* my_value_exps = a.scales + page_size + lane % 16;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int y = (lane + i * kWave) % D;
+    // (a multiple of 64 elements: the same for every lane)
+    more_k[i] = D % 64 == 0 ? i * 64 * page_size : (y / 32 - lane % D / 32) * page_size * 32;
+    more_v[i] = D % 64 == 0 ? i * 64 * page_size : (y - lane % D) * page_size;
+    k_at[i] = static_cast<uint32_t>((member * DB + y / 32) * 1024 + block_key * 64 + ((y % 2 * 2) ^ (block_key / 4)) * 16);  // (the other half: ^ 16)
+    v_at[i] = static_cast<uint32_t>((member * DB + y / 32) * 1024 + y % 32 * 32 + (y % 32 / 8 % 2) * 16);                    // (the other half: ^ 16)
+  }
+  // Pages are asked for a turn before the codes, by vector loads although a wavefront's is one: loads of the scalar unit share a
+  // counter with the reads of LDS, and every barrier would wait for them.  Addresses are formed in vector registers too, in one
+  // instruction each: with one or two wavefronts on a SIMD unit it is the number of instructions of any kind that counts.
+  uint32_t no_lane = 0;  // 0, which the compiler cannot know to be the same in every lane
+  asm("" : "+v"(no_lane));
+  auto first_of = [&](int chunk) {  // a block that the sequence holds
+    int key = key_begin + 64 * (chunk < nchunks ? chunk : nchunks - 1) + member * 16;
+    key = key > lo_min ? key : lo_min;
+    return key < pos_max ? key : pos_max;
   };
-  auto piece = [&](int i) { return (wave * kWave + lane + i * kThreads) % (2 * kPieces); };
-  auto is_key = [&](int i) { return (wave * kWave + i * kThreads) % (2 * kPieces) < kPieces; };
-  auto fetch = [&](Held (&held)[kPer], int chunk) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int x = piece(i) % kPieces, y = x % D;
-      int key = key_begin + 64 * (chunk < nchunks ? chunk : nchunks - 1) + x / D * 16;
-      key = key > lo_min ? key : lo_min;  // a block that the sequence holds
-      key = key < pos_max ? key : pos_max;
-      if (D % 64 == 0) key = __builtin_amdgcn_readfirstlane(key);  // (a wavefront's pieces are of one block)
-      const int entry = pd.div(key), slot = (key - entry * a.page_size) & ~15;
-      const int page = table[entry < a.table_stride ? entry : a.table_stride - 1];
-      const size_t part = static_cast<size_t>(page >= 0 && page < a.num_pages ? page : 0) * a.kv_heads + kvh;  // (never outside the pool)
-      if (is_key(i)) {
-        const int of_block = y % 32 / 2;
-        held[i].codes = *reinterpret_cast<const u32x4*>(a.k_pool + part * row_bytes + static_cast<size_t>(y / 32) * a.page_size * 32 +
-                                                         (slot + of_block) * 32 + y % 2 * 16);
-        held[i].exps[0] = a.scales[part * 2 * a.page_size + slot + of_block];
-      } else {
-        held[i].codes = *reinterpret_cast<const u32x4*>(a.v_pool + part * row_bytes + static_cast<size_t>(y) * a.page_size + slot);
-        held[i].exps = *reinterpret_cast<const u32x4*>(a.scales + (part * 2 + 1) * a.page_size + slot);
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
+  auto find = [&](int chunk) __attribute__((always_inline)) {
+    const int entry = PAGE ? first_of(chunk) / (PAGE ? PAGE : 1) : pd.div(first_of(chunk));
+    const uint32_t at = static_cast<uint32_t>(entry < a.table_stride ? entry : a.table_stride - 1) * 4 + no_lane;
+    return *reinterpret_cast<const int32_t*>(reinterpret_cast<const char*>(table) + at);
   };
-  auto put = [&](const Held (&held)[kPer], int chunk, int buf) {
-    char* keys = reinterpret_cast<char*>(&mem[buf][0]);
-    char* values = keys + kSide;
+  struct Place {  // where a block begins: its head's part of a page (never outside the pool), its first slot there
+    uint32_t part;
+    int slot;
+  };
+  auto place_of = [&](int page, int chunk) __attribute__((always_inline)) {
+    const uint32_t last = static_cast<uint32_t>(a.num_pages) - 1, inside = static_cast<uint32_t>(page) < last ? page : last;
+    return Place{inside * static_cast<uint32_t>(a.kv_heads) + kvh, PAGE == 16 ? 0 : pd.mod(first_of(chunk)) & ~15};
+  };
+  struct Codes {
+    u32x4 piece[kPer];
+    uint32_t exp;  // of keys: of the pieces' key; of values: of key lane % 16
+  };
+  char* const keys = reinterpret_cast<char*>(&mem[team][0]);  // two chunks of them
+  char* const values = keys + 2 * kSide;                      // and two of the values
+  Codes next_keys, next_values;  // as they come from the pages, of the next chunk or the one after
+  bf16x8 ready[2 * kPer];        // the next chunk's values, before they go to LDS
+  auto fetch_keys = [&](const Place& at) __attribute__((always_inline)) {
+    const uint8_t* from = my_keys + static_cast<uint64_t>(at.part) * row_bytes + at.slot * 32;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int x = piece(i) % kPieces, y = x % D, blk = x / D;
-      const u32x4 w = held[i].codes;
-      if (is_key(i)) {
-        const int of_block = y % 32 / 2;
-        const float unit = __uint_as_float(held[i].exps[0] << 23);
-        char* at = keys + (blk * DB + y / 32) * 1024 + of_block * 64;
+    for (int i = 0; i < kPer; ++i) next_keys.piece[i] = *reinterpret_cast<const u32x4*>(from + static_cast<int>(more_k[i]));
+    next_keys.exp = *(my_key_exps + static_cast<uint64_t>(at.part) * (2u * page_size) + at.slot);
+  };
+  auto fetch_values = [&](const Place& at) __attribute__((always_inline)) {
+    const uint8_t* from = my_values + static_cast<uint64_t>(at.part) * row_bytes + at.slot;
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
-          *reinterpret_cast<bf16x8*>(at + ((y % 2 * 2 + p) ^ (of_block / 4)) * 16) = bf16_of_codes(w[2 * p], w[2 * p + 1], unit);
-      } else {
-        char* at = values + (blk * DB + y / 32) * 1024 + y % 32 * 32;
-        const int first = key_begin + 64 * chunk + blk * 16;
-        const bool edge = first < lo_min || first + 15 > pos_max;
+    for (int i = 0; i < kPer; ++i) next_values.piece[i] = *reinterpret_cast<const u32x4*>(from + static_cast<int>(more_v[i]));
+    next_values.exp = *(my_value_exps + static_cast<uint64_t>(at.part) * (2u * page_size) + at.slot);
+  };
+  // half h of a piece i of the next chunk's keys to LDS; of its values into `ready`
+  auto put_keys = [&](int slot, int i, int h) __attribute__((always_inline)) {
+    const u32x4 w = next_keys.piece[i];
+    *reinterpret_cast<bf16x8*>(keys + slot * kSide + (k_at[i] ^ (h * 16))) =
+        bf16_of_codes(w[2 * h], w[2 * h + 1], __uint_as_float(next_keys.exp << 23));
+  };
+  auto ready_values = [&](int i, int h) __attribute__((always_inline)) {
+    const u32x4 w = next_values.piece[i];
+    ready[2 * i + h] = bf16_of_codes(w[2 * h], w[2 * h + 1], 1.f);
+  };
+  float ready_unit;
+  auto put_values = [&](int chunk, int slot) __attribute__((always_inline)) {
+    const int first = key_begin + 64 * chunk + member * 16;
+    if (first < lo_min || first + 15 > pos_max) {  // (kept a branch)
+      asm volatile("");
+      // slots that no query reads may hold anything, NaN and an infinite unit among them, and their weights of 0 times that have to be 0
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          bf16x8 v;
+      for (int h = 0; h < 2; ++h) {
+        u32x4 keep;
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const int word = 2 * p + e / 4;
-            const auto pair = e % 4 ? __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[word]), true)
-                                    : __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[word]), false);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              float f = pair[b] * __uint_as_float((held[i].exps[word] >> ((e % 4 + b) * 8) & 0xffu) << 23);
-              // a slot that no query reads may hold anything, and its weight of 0 times that has to be 0
-              const int key = first + 8 * p + e + b;
-              if (edge && (key < lo_min || key > pos_max)) f = 0.f;
-              v[e + b] = static_cast<__bf16>(f);
-            }
-          }
-          *reinterpret_cast<bf16x8*>(at + (p ^ (y % 32 / 8 % 2)) * 16) = v;
+        for (int e = 0; e < 4; ++e) {
+          const int at = first + 8 * h + 2 * e;
+          keep[e] = (at < lo_min || at > pos_max ? 0u : 0xffffu) | (at + 1 < lo_min || at + 1 > pos_max ? 0u : 0xffff0000u);
         }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          ready[2 * i + h] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, ready[2 * i + h]) & keep);
       }
+      if (first + lane % 16 < lo_min || first + lane % 16 > pos_max) ready_unit = 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) *reinterpret_cast<bf16x8*>(values + slot * kSide + (v_at[i] ^ (h * 16))) = ready[2 * i + h];
+    units[team][slot][member * 16 + lane % 16] = ready_unit;
   };
 
   // ---- where this lane's operands lie
   const int key = 16 * (col / 16) + 8 * (col / 4 % 2) + 4 * (col / 8 % 2) + col % 4;  // of a tile's 32: its row `col`
   const int turn = key % 16 / 4;
-  const int kat = key / 16 * DB * 1024 + key % 16 * 64, vat = kSide + col * 32 + (half ^ (col / 8 % 2)) * 16;
+  const int kat = key / 16 * DB * 1024 + key % 16 * 64, vat = col * 32 + (half ^ (col / 8 % 2)) * 16;
 
   const int last_plain = (pos_min + 1 - key_begin) / 64 - 1;  // the last chunk that every query reads whole, and the first
   const int first_plain = lo_max > key_begin ? (lo_max - key_begin + 63) / 64 : 0;
-  auto attend = [&](int buf, int chunk) {
-    const char* lds = reinterpret_cast<const char*>(&mem[buf][0]);
-    f32x16 s[2];
+  f32x16 s[2];
+  bf16x8 p[4];
+  auto add_values = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int q = 0; q < 4 * DB; ++q) {
+      const bf16x8 vf = *reinterpret_cast<const bf16x8*>(values + slot * kSide + vat + q * 1024);
+      o[q % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, p[q / DB], o[q % DB], 0, 0, 0);
+    }
+  };
+  // ---- the multiplications of a turn: the weights of the turn before with their values (not in the first turn), then the scores
+  // of the keys in `slot`.  Operands are read kAhead multiplications before their own; between them what there is to do for
+  // the next chunks, piece by piece.  Nothing moves across sched_barrier.
+  constexpr int kAhead = 4;
+  auto multiply = [&](int slot, int page_ahead, int chunk_ahead, auto with_values) __attribute__((always_inline)) {
+    constexpr int kValues = decltype(with_values)::value ? 4 * DB : 0, kSteps = kValues + 2 * KS;
+    constexpr int kItems = 4 * kPer + 4;
+    const char* from_keys = keys + slot * kSide + kat;
+    const char* from_values = values + (1 - slot) * kSide + vat;
+    bf16x8 operand[kSteps];
+    auto ask = [&](int q) __attribute__((always_inline)) {
+      if (q < kValues) {
+        operand[q] = *reinterpret_cast<const bf16x8*>(from_values + q * 1024);
+      } else {  // the two tiles by turns
+        const int t = (q - kValues) % 2, st = (q - kValues) / 2;
+        operand[q] = *reinterpret_cast<const bf16x8*>(from_keys + 2 * t * DB * 1024 + st / 2 * 1024 + ((st % 2 * 2 + half) ^ turn) * 16);
+      }
+    };
+    Place at;
+    int found = 0;
+    auto item = [&](int k) __attribute__((always_inline)) {
+      if (k < 2 * kPer) ready_values(k / 2, k % 2);
+      else if (k < 4 * kPer) put_keys(1 - slot, k / 2 - kPer, k % 2);
+      else if (k == 4 * kPer) ready_unit = __uint_as_float(next_values.exp << 23), at = place_of(page_ahead, chunk_ahead);
+      else if (k == 4 * kPer + 1) found = find(chunk_ahead + TEAMS);
+      else if (k == 4 * kPer + 2) fetch_keys(at);
+      else fetch_values(at);
+    };
+    if constexpr (TEAMS == 1) {
+      // (heads of more than 128 elements: so many steps that the compiler would rather keep their operands in memory than unroll
+      // them all with their items between them)
+      if (kValues) add_values(1 - slot);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+#pragma unroll
+        for (int st = 0; st < KS; ++st)
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              *reinterpret_cast<const bf16x8*>(from_keys + 2 * t * DB * 1024 + st / 2 * 1024 + ((st % 2 * 2 + half) ^ turn) * 16), qf[st], s[t], 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) item(k);
+      return found;
+    }
+#pragma unroll
+    for (int q = 0; q < kAhead && q < kSteps; ++q) ask(q);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+    // before the other team's wavefront, whose vector instructions would keep this one's multiplications waiting
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int st = 0; st < KS; ++st) {
-        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(lds + 2 * t * DB * 1024 + kat + st / 2 * 1024 + ((st % 2 * 2 + half) ^ turn) * 16);
-        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st], s[t], 0, 0, 0);
+    for (int q = 0; q < kSteps; ++q) {
+      if (q + kAhead < kSteps) ask(q + kAhead);
+      if (q < kValues) {
+        o[q % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand[q], p[q / DB], o[q % DB], 0, 0, 0);
+      } else {
+        const int t = (q - kValues) % 2, st = (q - kValues) / 2;
+        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand[q], qf[st], s[t], 0, 0, 0);
       }
+#pragma unroll
+      for (int k = 0; k < kItems; ++k)
+        if (k * kSteps / kItems == q) item(k);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
+    return found;
+  };
+  auto weigh = [&](int chunk, int slot) __attribute__((always_inline)) {
     const int kb = key_begin + 64 * chunk;
     if (chunk > last_plain || chunk < first_plain) {  // some query does not read all of it
       asm volatile("");  // (stays a branch)
@@ -579,63 +688,114 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attention_port
           if (at > q_pos || at < q_lo) s[t][e] = -INFINITY;
         }
     }
-    float mx = fmaxf(s[1][0], s[1][1]);
+    float sum;
+    auto weights = [&]() __attribute__((always_inline)) {
+      float part[2] = {0.f, 0.f};
+      const float* unit = &units[team][slot][8 * half];
 #pragma unroll
-    for (int e = 2; e < 16; ++e) mx = fmaxf(mx, s[1][e]);
+      for (int u = 0; u < 4; ++u) {  // eight keys of a block
+        const f32x4 by[2] = {*reinterpret_cast<const f32x4*>(unit + 16 * u), *reinterpret_cast<const f32x4*>(unit + 16 * u + 4)};
 #pragma unroll
-    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[0][e]);
-    {
+        for (int e = 0; e < 8; ++e) {
+          const float w = __builtin_amdgcn_exp2f(fmaf(s[u / 2][u % 2 * 8 + e], scale2, shift));
+          part[e % 2] += w;
+          p[u][e] = static_cast<__bf16>(w * by[e / 4][e % 4]);
+        }
+      }
+      sum = part[0] + part[1];
+    };
+    weights();
+    // The reference is some earlier chunk's maximum.  It only has to keep weights in float32's range: a weight of 2^10 is as exact as
+    // one of 1.  So the maximum is not looked for as long as a row's weights stay small, and o is not rescaled.
+    if (__builtin_amdgcn_ballot_w64(sum > limit) != 0) {
+      asm volatile("");
+      float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(fmaxf(mx, s[0][e]), s[1][e]);
       const unsigned b = __builtin_bit_cast(unsigned, mx);
       const auto halves = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-      mx = fmaxf(bits_as_float(halves[0]), bits_as_float(halves[1]));
-    }
-    const float m_new = fmaxf(m, mx);
-    const float m_safe = m_new == -INFINITY ? 0.f : m_new;  // (a row that has read no key yet)
-    const float alpha = __builtin_amdgcn_exp2f((m - m_safe) * scale2), shift = -m_safe * scale2;
-    m = m_new;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    bf16x8 p[4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float w = __builtin_amdgcn_exp2f(fmaf(s[t][e], scale2, shift));
-        sum[e % 4] += w;
-        p[2 * t + e / 8][e % 8] = static_cast<__bf16>(w);
-      }
-    l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {  // some row's maximum rose
+      const float m_new = fmaxf(m, fmaxf(bits_as_float(halves[0]), bits_as_float(halves[1])));
+      const float m_safe = m_new == -INFINITY ? 0.f : m_new;  // (a row that has read no key yet)
+      const float alpha = __builtin_amdgcn_exp2f((m - m_safe) * scale2);
+      m = m_new;
+      shift = -m_safe * scale2;
+      limit = m == -INFINITY ? -1.f : kLargeSum;  // (a row without a reference: any sum is over it)
+      l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
+      weights();
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const bf16x8 vf = *reinterpret_cast<const bf16x8*>(lds + vat + (u * DB + db) * 1024);
-        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, p[u], o[db], 0, 0, 0);
-      }
+    l += sum;
   };
 
   if (c_first < c_end) {  // the same for every wavefront of the workgroup
-    Held held[kPer];
-    fetch(held, c_first);
-    put(held, c_first, 0);
-    fetch(held, c_first + 1);
-    for (int c = c_first; c < c_end; ++c) {
-      const int buf = (c - c_first) % 2;
-      __syncthreads();  // chunk c is in LDS, and nobody reads chunk c - 1 any more
-      attend(buf, c);
-      put(held, c + 1, 1 - buf);  // (behind the last chunk: the last block again, which nobody reads)
-      fetch(held, c + 2);
+    // the team's chunks: c_first + team, + TEAMS, ...; every team takes part in every turn's barriers
+    const int turns = (c_end - c_first + TEAMS - 1) / TEAMS;
+    auto chunk_of = [&](int turn_) { return c_first + team + TEAMS * turn_; };
+    int page = find(chunk_of(0));
+    Place at = place_of(page, chunk_of(0));
+    fetch_keys(at);
+    fetch_values(at);
+    page = find(chunk_of(1));
+#pragma unroll
+    for (int i = 0; i < 2 * kPer; ++i) put_keys(0, i / 2, i % 2), ready_values(i / 2, i % 2);
+    ready_unit = __uint_as_float(next_values.exp << 23);
+    put_values(chunk_of(0), 0);
+    at = place_of(page, chunk_of(1));
+    fetch_keys(at);
+    fetch_values(at);
+    page = find(chunk_of(2));
+    __syncthreads();
+    if (TEAMS == 2 && team == 1) __syncthreads();  // half a turn behind
+    // (a team without a chunk in the last turn forms scores of the last block again, which are not used)
+    auto rest = [&](int i) __attribute__((always_inline)) {
+      __syncthreads();  // the team has read the values of the turn before
+      put_values(chunk_of(i + 1), (i + 1) % 2);
+      if (chunk_of(i) < c_end) weigh(chunk_of(i), i % 2);
+      __syncthreads();
+    };
+    page = multiply(0, page, chunk_of(2), EdgeTag<false>{});
+    rest(0);
+    for (int i = 1; i < turns; ++i) {
+      page = multiply(i % 2, page, chunk_of(i + 2), EdgeTag<true>{});
+      rest(i);
     }
+    if (chunk_of(turns - 1) < c_end) add_values((turns - 1) % 2);
+    if (TEAMS == 2 && team == 0) __syncthreads();
   }
 
-  float total = l;
+  float total;
   {
     const unsigned b = __builtin_bit_cast(unsigned, l);
     const auto halves = __builtin_amdgcn_permlane32_swap(b, b, false, false);
     total = bits_as_float(halves[0]) + bits_as_float(halves[1]);
+  }
+  if (TEAMS == 2) {
+    // ---- the teams' results become one
+    __syncthreads();
+    f32x4* sums = reinterpret_cast<f32x4*>(&mem[0][0]);
+    if (team == 1) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          sums[(member * DB * 4 + db * 4 + g) * kWave + lane] = f32x4{o[db][g * 4], o[db][g * 4 + 1], o[db][g * 4 + 2], o[db][g * 4 + 3]};
+      if (!half) ends[1][0][row] = m, ends[1][1][row] = total;
+    }
+    __syncthreads();
+    if (team == 1) return;
+    const float other = ends[1][0][row], top = fmaxf(m, other), ref = top == -INFINITY ? 0.f : top;
+    const float mine_by = __builtin_amdgcn_exp2f((m - ref) * scale2), other_by = __builtin_amdgcn_exp2f((other - ref) * scale2);
+    total = total * mine_by + ends[1][1][row] * other_by;
+    m = top;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = sums[(member * DB * 4 + db * 4 + g) * kWave + lane];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[db][g * 4 + r] = o[db][g * 4 + r] * mine_by + x[r] * other_by;
+      }
   }
   if (!mine) return;
   if (a.nsplit > 1) {
@@ -649,8 +809,7 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attention_port
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<f32x4*>(dst + db * 32 + g * 8) = f32x4{o[db][g * 4], o[db][g * 4 + 1], o[db][g * 4 + 2], o[db][g * 4 + 3]};
     if (!half)
-      *reinterpret_cast<float2*>(a.partial + rows * a.nsplit * D + (at * a.nsplit + z) * 2) =
-          make_float2(m * scale2, total);
+      *reinterpret_cast<float2*>(a.partial + rows * a.nsplit * D + (at * a.nsplit + z) * 2) = make_float2(m * scale2, total);
     return;
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;  // (a query that reads no key: zeros)
@@ -725,14 +884,14 @@ void merge_e4m3(int rows, hipStream_t s, const float* partial, void* out, int ns
 
 #define E4M3_BY_DIM(head_dim, CASE) \
   switch (head_dim) {               \
-    case 32: CASE(32); break;       \
-    case 64: CASE(64); break;       \
-    case 96: CASE(96); break;       \
-    case 128: CASE(128); break;     \
-    case 160: CASE(160); break;     \
-    case 192: CASE(192); break;     \
-    case 224: CASE(224); break;     \
-    case 256: CASE(256); break;     \
+    case 32: { CASE(32); } break;    \
+    case 64: { CASE(64); } break;    \
+    case 96: { CASE(96); } break;    \
+    case 128: { CASE(128); } break;  \
+    case 160: { CASE(160); } break;  \
+    case 192: { CASE(192); } break;  \
+    case 224: { CASE(224); } break;  \
+    case 256: { CASE(256); } break;  \
   }
 
 }  // namespace
@@ -787,20 +946,20 @@ extern "C" int shk_attention_prefill_e4m3(const void* q, int q_stride, void* out
               "attention_prefill_e4m3: rows must be 16-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int tokens = n - first_seq, group = heads / kv_heads;
-  auto groups = [&](int rows) { return static_cast<long long>(tokens / (rows / group) + num_seqs) * kv_heads * nsplit; };
-  const bool wide = head_dim <= 128 && groups(256) >= 256;
-  const long long count = groups(wide ? 256 : 128);
+  const int queries = kPortionRows / group;
+  const long long count = static_cast<long long>(tokens / queries + num_seqs) * kv_heads * nsplit;
   SHK_REQUIRE(count < (1LL << 31) && static_cast<long long>(tokens) * heads < (1LL << 31), "attention_prefill_e4m3: too many tokens: %d",
               tokens);
+  SHK_REQUIRE(static_cast<long long>(num_pages) * kv_heads < (1LL << 31) && static_cast<long long>(page_size) * head_dim < (1LL << 31),
+              "attention_prefill_e4m3: %d pages of %d are too many", num_pages, page_size);
   const PortionArgs a{static_cast<const bf16*>(q), static_cast<bf16*>(out), cu_q, ctx_lens, tables, static_cast<const uint8_t*>(k_pool),
                       static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(scales), partial, n, q_stride, heads, kv_heads,
-                      (wide ? 256 : 128) / group, first_seq, num_seqs, table_stride, page_size, num_pages, window, chunk, nsplit,
+                      queries, first_seq, num_seqs, table_stride, page_size, num_pages, window, chunk, nsplit,
                       page_magic(page_size), scale};
-#define LAUNCH(D)                                                                                                          \
-  if (wide)                                                                                                                \
-    attention_portion_e4m3_kernel<(D <= 128 ? D : 32), 8><<<static_cast<unsigned>(count), 8 * kWave, 0, s>>>(a);           \
-  else                                                                                                                     \
-    attention_portion_e4m3_kernel<D, 4><<<static_cast<unsigned>(count), 4 * kWave, 0, s>>>(a);                             \
+#define LAUNCH(D)                                                                                                       \
+  constexpr int kTeams##D = D <= 128 ? 2 : 1;                                                                           \
+  (page_size == 16 ? attention_portion_e4m3_kernel<D, kTeams##D, 16> : attention_portion_e4m3_kernel<D, kTeams##D, 0>)   \
+      <<<static_cast<unsigned>(count), kTeams##D * 4 * kWave, 0, s>>>(a);                                               \
   if (nsplit > 1) merge_e4m3<D>(tokens * heads, s, partial, static_cast<bf16*>(out) + static_cast<size_t>(first_seq) * heads * D, nsplit)
   E4M3_BY_DIM(head_dim, LAUNCH)
 #undef LAUNCH
