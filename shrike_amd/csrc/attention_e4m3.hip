@@ -114,12 +114,12 @@ __device__ __forceinline__ bf16x8 bf16_of_codes(uint32_t lo, uint32_t hi, float 
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-template <int D, int WAVES>
-__global__ void __launch_bounds__(WAVES* kWave)
+template <int D, int WAVES, int PAGE>
+__global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
     attention_decode_e4m3_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict__ out, int heads, int head_tiles,
                                  const int32_t* __restrict__ positions, const int32_t* __restrict__ tables, int table_stride,
                                  const uint8_t* __restrict__ k_pool, const uint8_t* __restrict__ v_pool,
-                                 const uint8_t* __restrict__ scales, int kv_heads, int page_size, uint32_t page_magic, int num_pages,
+                                 const uint8_t* __restrict__ scales, int kv_heads, int any_page_size, uint32_t page_magic, int num_pages,
                                  int window, int block, float scale, float* __restrict__ partial, int nsplit) {
   constexpr int kStep = 64 * WAVES;  // keys between two chunks of one wavefront
   constexpr int kPairs = D / 64, kOdd = D / 32 % 2;
@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(WAVES* kWave)
   const int group = heads / kv_heads;
   const int first_head = kvh * group + blockIdx.x % head_tiles * 16;  // of this workgroup's tile
   const int tile_heads = min(16, kvh * group + group - first_head);
+  const int page_size = PAGE ? PAGE : any_page_size;
   const PageDiv pd{page_size, page_magic};
   const int pos = positions[seq], lo = first_key(pos, window, block);
   const int first = lo & ~63;
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(WAVES* kWave)
       return kb > pos ? pos & ~15 : kb;
     };
     auto page_of = [&](int kb) {
-      const int entry = pd.div(clamped_block(kb));
+      const int entry = PAGE ? clamped_block(kb) / (PAGE ? PAGE : 1) : pd.div(clamped_block(kb));
       const int page = table[entry < table_stride ? entry : table_stride - 1];
       return page >= 0 && page < num_pages ? page : 0;  // (an id outside the pool is never followed)
     };
@@ -176,10 +177,11 @@ __global__ void __launch_bounds__(WAVES* kWave)
       int k, v;
     };
     auto find = [&](int kb) { return Pages{page_of(kb + j / 4 * 16), page_of(kb + g * 16)}; };
-    auto fetch = [&](CodeChunk<D>& c, int kb, Pages at) {
-      const int k_slot = pd.mod(clamped_block(kb + j / 4 * 16)), v_slot = pd.mod(clamped_block(kb + g * 16));
-      const size_t k_part = static_cast<size_t>(at.k) * kv_heads + kvh, v_part = static_cast<size_t>(at.v) * kv_heads + kvh;
-      const uint8_t* key = k_pool + k_part * row_bytes + static_cast<size_t>(k_slot + j % 4) * 32;
+    CodeChunk<D> c;
+    auto fetch_keys = [&](int kb, Pages at) {
+      const int slot = PAGE == 16 ? 0 : pd.mod(clamped_block(kb + j / 4 * 16));
+      const size_t part = static_cast<size_t>(at.k) * kv_heads + kvh;
+      const uint8_t* key = k_pool + part * row_bytes + static_cast<size_t>(slot + j % 4) * 32;
       const uint8_t* pair = key + static_cast<size_t>(g / 2) * page_size * 32 + g % 2 * 16;
       const uint8_t* odd = key + static_cast<size_t>(2 * kPairs) * page_size * 32 + g * 8;
 #pragma unroll
@@ -189,14 +191,20 @@ __global__ void __launch_bounds__(WAVES* kWave)
           c.k[t].pair[i] = *reinterpret_cast<const u32x4*>(pair + t * 128 + static_cast<size_t>(i) * page_size * 64);
         if (kOdd) c.k[t].odd = *reinterpret_cast<const uint2*>(odd + t * 128);
       }
-      const uint8_t* value = v_pool + v_part * row_bytes + static_cast<size_t>(j) * page_size + v_slot;
+      c.k_exp = *reinterpret_cast<const u32x4*>(scales + part * 2 * page_size + slot);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto fetch_values = [&](int kb, Pages at) {
+      const int slot = PAGE == 16 ? 0 : pd.mod(clamped_block(kb + g * 16));
+      const size_t part = static_cast<size_t>(at.v) * kv_heads + kvh;
+      const uint8_t* value = v_pool + part * row_bytes + static_cast<size_t>(j) * page_size + slot;
 #pragma unroll
       for (int db = 0; db < D / 16; ++db) c.v[db] = *reinterpret_cast<const u32x4*>(value + static_cast<size_t>(db) * 16 * page_size);
-      c.k_exp = *reinterpret_cast<const u32x4*>(scales + k_part * 2 * page_size + k_slot);
-      c.v_exp = *reinterpret_cast<const u32x4*>(scales + (v_part * 2 + 1) * page_size + v_slot);
+      c.v_exp = *reinterpret_cast<const u32x4*>(scales + (part * 2 + 1) * page_size + slot);
+      __builtin_amdgcn_sched_barrier(0);
     };
 
-    auto attend_chunk = [&](const CodeChunk<D>& c, int kb, auto edge_tag) {
+    auto attend_chunk = [&](int kb, int next_kb, Pages next, auto edge_tag) {
       constexpr bool edge = decltype(edge_tag)::value;
       f32x4 s[4];
 #pragma unroll
@@ -213,6 +221,7 @@ __global__ void __launch_bounds__(WAVES* kWave)
         if (kOdd)
           s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(c.k[t].odd.x, c.k[t].odd.y, unit), qf[D / 32 - 1], s[t], 0, 0, 0);
       }
+      fetch_keys(next_kb, next);
       // this lane's keys are kb + 16 g + e, e = 4 t + r
       const int g0 = kb + g * 16;
       float sc[16];
@@ -265,29 +274,22 @@ __global__ void __launch_bounds__(WAVES* kWave)
         o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(v[2], v[3], 1.f), pf[1], o[db], 0, 0, 0);
       }
     };
-    auto attend = [&](const CodeChunk<D>& c, int kb) {
-      if (kb + 63 > pos || kb < lo)  // wave-uniform
-        attend_chunk(c, kb, EdgeTag<true>{});
-      else
-        attend_chunk(c, kb, EdgeTag<false>{});
-    };
-
-    // One chunk's loads are in flight while the chunk before is computed, and the pages of the one after; every step issues the
-    // same loads (past the end the last chunk's again), so that the compiler can count them.
+    // The next chunk's keys are asked for when this one's have become scores, its values when this one's have been added, its
+    // pages a chunk before; every step issues the same loads (past the end the last chunk's again).
     const int last = key_begin + (key_end - 1 - key_begin) / kStep * kStep;
     auto clamped = [&](int kb) { return kb < last ? kb : last; };
-    CodeChunk<D> buf[2];
-    fetch(buf[0], key_begin, find(key_begin));
-    Pages next = find(clamped(key_begin + kStep));
-    for (int kb0 = key_begin; kb0 < key_end; kb0 += 2 * kStep) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int kb = kb0 + kStep * u;
-        if (kb >= key_end) break;
-        fetch(buf[1 - u], clamped(kb + kStep), next);
-        next = find(clamped(kb + 2 * kStep));
-        attend(buf[u], kb);
-      }
+    Pages next = find(key_begin);
+    fetch_keys(key_begin, next);
+    fetch_values(key_begin, next);
+    next = find(clamped(key_begin + kStep));
+    for (int kb = key_begin; kb < key_end; kb += kStep) {
+      const Pages after = find(clamped(kb + 2 * kStep));
+      if (kb + 63 > pos || kb < lo)  // wave-uniform
+        attend_chunk(kb, clamped(kb + kStep), next, EdgeTag<true>{});
+      else
+        attend_chunk(kb, clamped(kb + kStep), next, EdgeTag<false>{});
+      fetch_values(clamped(kb + kStep), next);
+      next = after;
     }
     l = lanes4_sum(l);
   }
@@ -918,7 +920,7 @@ extern "C" int shk_attention_decode_e4m3(const void* q, int q_stride, void* out,
   const int head_tiles = (heads / kv_heads + 15) / 16;
   const dim3 grid(kv_heads * head_tiles, num_seqs, nsplit);
 #define LAUNCH(D)                                                                                                                \
-  attention_decode_e4m3_kernel<D, 4><<<grid, 4 * kWave, 0, s>>>(                                                                 \
+  (page_size == 16 ? attention_decode_e4m3_kernel<D, 4, 16> : attention_decode_e4m3_kernel<D, 4, 0>)<<<grid, 4 * kWave, 0, s>>>( \
       static_cast<const bf16*>(q), q_stride, static_cast<bf16*>(out), heads, head_tiles, positions, tables, table_stride,        \
       static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(scales), kv_heads,   \
       page_size, page_magic(page_size), num_pages, window, chunk, scale, partial, nsplit);                                       \

@@ -6,7 +6,8 @@
 namespace shk {
 
 constexpr int kStoreThreads = 256, kStoreWaves = kStoreThreads / kWave;
-constexpr int kMaxDim = 256, kPerLane = kMaxDim / kWave;
+constexpr int kMaxDim = 256;
+constexpr int kManyTokens = 65;
 
 struct StoreArgs {
   const void* qkv;      // [n, width], or null with parts
@@ -19,90 +20,306 @@ struct StoreArgs {
   float magnitude;
 };
 
-// Cosines and sines of a token's angles into LDS.  The angle is formed in float64 and brought into [-pi, pi] there: at position
+// Cosine and sine of a token's angle, times `magnitude`.  The angle is formed in float64 and brought into [-pi, pi] there: at position
 // 16,000 a float32 product is off by up to 5e-4 radians, which would move one code in a thousand.
-__device__ __forceinline__ void tabulate(const StoreArgs& a, int pos, float* cs, float* sn) {
-  for (int f = threadIdx.x; f < a.rot_dim / 2; f += kStoreThreads) {
-    const double angle = static_cast<double>(pos) * static_cast<double>(a.inv_freq[f]);
-    const double turns = rint(angle * 0.15915494309189535);
-    float s, c;
-    sincosf(static_cast<float>(fma(turns, -6.283185307179586, angle)), &s, &c);
-    cs[f] = c * a.magnitude;
-    sn[f] = s * a.magnitude;
+__device__ __forceinline__ void turn_of(int pos, float inv_freq, float magnitude, float& c, float& s) {
+  const double angle = static_cast<double>(pos) * static_cast<double>(inv_freq);
+  const double turns = rint(angle * 0.15915494309189535);
+  sincosf(static_cast<float>(fma(turns, -6.283185307179586, angle)), &s, &c);
+  c *= magnitude;
+  s *= magnitude;
+}
+
+__device__ __forceinline__ uint32_t size_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// A wavefront per head of a token, four neighbouring heads a workgroup; any sizes, types and ways of pairing.  A lane owns pairs that
+// turn together (lane, lane + 64) and elements behind the rotated part, forms its own cosines and meets nobody but its
+// wavefront: what a step of single tokens costs is the way of its loads.  (One workgroup per token, its heads one after the other, with
+// a table of cosines: 8 tokens of 28 heads over 4 11.1 us, 4.5 so.)
+template <typename T>
+__global__ void __launch_bounds__(kStoreThreads) store_e4m3_kernel(StoreArgs a, E4m3Pools pools, int row_groups) {
+  const int t = blockIdx.x / row_groups, lane = threadIdx.x % kWave;
+  const int r = __builtin_amdgcn_readfirstlane(blockIdx.x % row_groups * kStoreWaves + threadIdx.x / kWave);
+  const int dim = a.head_dim, half = a.rot_dim / 2, width = (a.heads + (a.v_from_k ? 1 : 2) * a.kv_heads) * dim;
+  if (r >= a.heads + (a.write_kv ? 2 * a.kv_heads : 0)) return;
+  // heads of the queries, then of the keys, then of the values
+  const bool value = r >= a.heads + a.kv_heads;
+  const int from = (value && a.v_from_k ? r - a.kv_heads : r) * dim, turned = value ? 0 : a.rot_dim;
+  const int pos = a.positions[t];
+  const T* row = static_cast<const T*>(a.qkv) + static_cast<size_t>(t) * width + from;
+  const size_t stride = static_cast<size_t>(a.n) * width;
+  const float* part = a.parts + static_cast<size_t>(t) * width + from;
+  // columns d1 and d2 of the row; the parts of a split product are added in order, four of each in flight
+  auto get2 = [&](int d1, int d2, float& x1, float& x2) {
+    if (a.splits == 0) {
+      x1 = to_float(row[d1]);
+      x2 = to_float(row[d2]);
+      return;
+    }
+    x1 = x2 = 0.f;
+    for (int z0 = 0; z0 < a.splits; z0 += 4) {
+      float u[4], v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const size_t at = stride * (z0 + k < a.splits ? z0 + k : a.splits - 1);
+        u[k] = part[at + d1];
+        v[k] = part[at + d2];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x1 += z0 + k < a.splits ? u[k] : 0.f;
+        x2 += z0 + k < a.splits ? v[k] : 0.f;
+      }
+    }
+    if (a.bias) {
+      x1 += a.bias[from + d1];
+      x2 += a.bias[from + d2];
+    }
+  };
+  // x[2 i], x[2 i + 1]: a pair that turns, or two elements that do not
+  constexpr int kPairs = kMaxDim / 2 / kWave;
+  float x[2 * kPairs];
+  int at[2 * kPairs];
+  const int tail = (dim - turned + 1) / 2;  // pairs of elements that do not turn: d and d + tail
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const int p = lane + i * kWave;
+    if (p < turned / 2) {
+      at[2 * i] = a.adjacent ? 2 * p : p;
+      at[2 * i + 1] = a.adjacent ? 2 * p + 1 : p + half;
+    } else {
+      const int d = turned + p - turned / 2;
+      at[2 * i] = d < turned + tail ? d : dim;
+      at[2 * i + 1] = d < turned + tail ? d + tail : dim;
+    }
+    get2(min(at[2 * i], dim - 1), min(at[2 * i + 1], dim - 1), x[2 * i], x[2 * i + 1]);
+  }
+  int page = -1;
+  if (r >= a.heads)
+    page = e4m3_page(a.tables, a.table_stride, a.num_seqs, a.token_seq[t], pos, pools.page_size, pools.num_pages);
+  uint32_t largest = 0;
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const int p = lane + i * kWave;
+    if (p < turned / 2) {
+      float c, s;
+      turn_of(pos, a.inv_freq[p], a.magnitude, c, s);
+      const float x1 = x[2 * i], x2 = x[2 * i + 1];
+      x[2 * i] = x1 * c - x2 * s;
+      x[2 * i + 1] = x2 * c + x1 * s;
+    }
+#pragma unroll
+    for (int e = 2 * i; e < 2 * i + 2; ++e) {
+      const uint32_t size = at[e] < dim ? size_bits(x[e]) : 0;
+      largest = size > largest ? size : largest;
+    }
+  }
+  if (r < a.heads) {  // (all of the row has been read: it may be written in place)
+    T* q_row = static_cast<T*>(a.q_out) + static_cast<size_t>(t) * a.q_ld + from;
+#pragma unroll
+    for (int e = 0; e < 2 * kPairs; ++e)
+      if (at[e] < dim) q_row[at[e]] = from_float<T>(x[e]);
+    return;
+  }
+  if (page < 0) return;
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) {
+    const uint32_t other = __shfl_xor(static_cast<int>(largest), off, kWave);
+    largest = other > largest ? other : largest;
+  }
+  const int byte = e4m3_exponent_byte(largest), slot = pos % pools.page_size;
+  const float inverse = e4m3_inverse_unit(byte);
+  const size_t where = pools.part(page, r - a.heads - (value ? a.kv_heads : 0)), base = where * pools.row_bytes();
+  if (lane == 0) pools.scales[(where * 2 + (value ? 1 : 0)) * pools.page_size + slot] = static_cast<uint8_t>(byte);
+#pragma unroll
+  for (int e = 0; e < 2 * kPairs; ++e) {
+    if (at[e] >= dim) continue;
+    const uint8_t code = e4m3_code(x[e], inverse, largest);
+    if (value)
+      pools.v[base + static_cast<size_t>(at[e]) * pools.page_size + slot] = code;
+    else
+      pools.k[base + key_offset(slot, at[e], pools.page_size, dim)] = code;
   }
 }
 
-// One workgroup per token, a wavefront per head at a time; any sizes, types and ways of pairing.
-template <typename T>
-__global__ void __launch_bounds__(kStoreThreads) store_e4m3_kernel(StoreArgs a, E4m3Pools pools) {
-  __shared__ float cs[kMaxDim / 2], sn[kMaxDim / 2];
-  const int t = blockIdx.x, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int pos = a.positions[t], half = a.rot_dim / 2, dim = a.head_dim;
-  const int width = (a.heads + (a.v_from_k ? 1 : 2) * a.kv_heads) * dim;
-  const T* row = static_cast<const T*>(a.qkv) + static_cast<size_t>(t) * width;
-  T* q_row = static_cast<T*>(a.q_out) + static_cast<size_t>(t) * a.q_ld;
-  const int page = a.write_kv ? e4m3_page(a.tables, a.table_stride, a.num_seqs, a.token_seq[t], pos, pools.page_size, pools.num_pages) : -1;
-  const int slot = page >= 0 ? pos % pools.page_size : 0;
-  tabulate(a, pos, cs, sn);
-  __syncthreads();
+// Many tokens of bfloat16 rows that turn whole, (i, i + head_dim / 2) together, head_dim a multiple of 32.  Queries and keys: a
+// workgroup per token, kLanes lanes a head with eight pairs each (16-byte loads, 8-byte pieces of codes) and a table of cosines.
+// Values: 16 neighbouring tokens of a step and one key/value head a workgroup; their codes turn in LDS, so that what lies side by side in a page
+// leaves in one piece, 16 bytes where the tokens fill a block of 16.  What bounds it is traffic: a token of 28 heads over 4 moves 17 KiB.
+constexpr int kBlock = 16;
 
-  auto get = [&](int col) {
-    if (a.splits == 0) return to_float(row[col]);
-    float x = 0.f;
-    for (int z = 0; z < a.splits; ++z) x += a.parts[(static_cast<size_t>(z) * a.n + t) * width + col];
-    return a.bias ? x + a.bias[col] : x;
+template <int LANES>
+__global__ void __launch_bounds__(kStoreThreads) store_many_e4m3_kernel(StoreArgs a, E4m3Pools pools, unsigned value_groups) {
+  __shared__ __attribute__((aligned(16))) float cs[kMaxDim / 2], sn[kMaxDim / 2];
+  __shared__ __attribute__((aligned(16))) uint8_t tile[kBlock][kMaxDim + 4];
+  const int dim = a.head_dim, half = dim / 2, width = (a.heads + 2 * a.kv_heads) * dim, tid = threadIdx.x;
+  const bf16* qkv = static_cast<const bf16*>(a.qkv);
+  const size_t stride = static_cast<size_t>(a.n) * width;
+  // eight elements from column `col` of row t on
+  auto fetch = [&](int t, int col, float (&x)[8]) {
+    if (a.splits == 0) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(qkv + static_cast<size_t>(t) * width + col);
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[2 * e] = __uint_as_float(w[e] << 16);
+        x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+      }
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    const float* p = a.parts + static_cast<size_t>(t) * width + col;
+    for (int z0 = 0; z0 < a.splits; z0 += 2) {  // two parts in flight, added in order
+      float4 v[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const size_t at = stride * (z0 + u < a.splits ? z0 + u : a.splits - 1);
+        v[u][0] = *reinterpret_cast<const float4*>(p + at);
+        v[u][1] = *reinterpret_cast<const float4*>(p + at + 4);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bool have = z0 + u < a.splits;
+        x[0] += have ? v[u][0].x : 0.f, x[1] += have ? v[u][0].y : 0.f, x[2] += have ? v[u][0].z : 0.f, x[3] += have ? v[u][0].w : 0.f;
+        x[4] += have ? v[u][1].x : 0.f, x[5] += have ? v[u][1].y : 0.f, x[6] += have ? v[u][1].z : 0.f, x[7] += have ? v[u][1].w : 0.f;
+      }
+    }
+    if (a.bias)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] += a.bias[col + e];
   };
-  // heads of the queries, then of the keys, then of the values
-  const int rows = a.heads + (page >= 0 ? 2 * a.kv_heads : 0);
-  for (int r = wave; r < rows; r += kStoreWaves) {
-    const bool value = r >= a.heads + a.kv_heads;
-    const int from = (value && a.v_from_k ? r - a.kv_heads : r) * dim;
-    float x[kPerLane];
+  auto codes = [&](const float (&x)[8], float inverse, uint32_t largest) {
+    const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
+    return make_uint2(e4m3_code4(lo, inverse, largest), e4m3_code4(hi, inverse, largest));
+  };
+  auto largest_of = [&](const float (&x)[8]) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = max(most, size_bits(x[e]));
+    return most;
+  };
+
+  if (blockIdx.x < value_groups) {
+    // ---- values: a token a row of 16 lanes or (heads of more than 128 elements) two rounds of them
+    const int head = blockIdx.x % a.kv_heads, first = blockIdx.x / a.kv_heads * kBlock;
+    const int mine = tid / 16, lane16 = tid % 16, t = first + mine;
+    const int token = min(t, a.n - 1), pos = a.positions[token];
+    const int page = t < a.n ? e4m3_page(a.tables, a.table_stride, a.num_seqs, a.token_seq[token], pos, pools.page_size, pools.num_pages) : -1;
+    const int slot = page >= 0 ? pos % pools.page_size : 0;
+    const int col = (a.heads + a.kv_heads + head) * dim;
+    float x[2][8];
     uint32_t largest = 0;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const int d = lane + i * kWave;
-      x[i] = 0.f;
+    for (int i = 0; i < 2; ++i) {
+      const int d = (lane16 + 16 * i) * 8;
       if (d >= dim) continue;
-      x[i] = get(from + d);
-      if (!value && d < a.rot_dim) {
-        const int pair = a.adjacent ? d / 2 : d % half;
-        const bool second = a.adjacent ? d % 2 : d >= half;
-        const int step = a.adjacent ? 1 : half;
-        const float y = get(from + (second ? d - step : d + step));
-        x[i] = second ? x[i] * cs[pair] + y * sn[pair] : x[i] * cs[pair] - y * sn[pair];
-      }
-      const uint32_t size = __float_as_uint(x[i]) & 0x7fffffffu;
-      largest = size > largest ? size : largest;
+      fetch(token, col + d, x[i]);
+      largest = max(largest, largest_of(x[i]));
     }
-    if (r < a.heads) {
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) {
-        const int d = lane + i * kWave;
-        if (d < dim) q_row[r * dim + d] = from_float<T>(x[i]);
+    for (int off = 8; off > 0; off >>= 1) largest = max(largest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(largest), off, 16)));
+    const int byte = e4m3_exponent_byte(largest);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = (lane16 + 16 * i) * 8;
+      if (d >= dim) continue;
+      const uint2 w = codes(x[i], e4m3_inverse_unit(byte), largest);
+      uint32_t* to = reinterpret_cast<uint32_t*>(&tile[mine][d]);  // (rows are a multiple of 4 bytes long)
+      to[0] = w.x;
+      to[1] = w.y;
+    }
+    if (lane16 == 0 && page >= 0)
+      pools.scales[(pools.part(page, head) * 2 + 1) * pools.page_size + slot] = static_cast<uint8_t>(byte);
+    int* pages = reinterpret_cast<int*>(cs);  // of the 16 tokens, then their slots
+    if (lane16 == 0) pages[mine] = page, pages[kBlock + mine] = slot;
+    __syncthreads();
+    if (tid >= dim) return;
+    // runs of tokens that are neighbours in a page, the same for every thread
+    for (int i = 0; i < kBlock;) {
+      const int run_page = __builtin_amdgcn_readfirstlane(pages[i]), run_slot = __builtin_amdgcn_readfirstlane(pages[kBlock + i]);
+      int len = 1;
+      while (i + len < kBlock && pages[i + len] == run_page && pages[kBlock + i + len] == run_slot + len) ++len;
+      if (run_page >= 0) {
+        uint8_t* to = pools.v + pools.part(run_page, head) * pools.row_bytes() + static_cast<size_t>(tid) * pools.page_size + run_slot;
+        auto four = [&](int k) {
+          return static_cast<uint32_t>(tile[i + k][tid]) | static_cast<uint32_t>(tile[i + k + 1][tid]) << 8 |
+                 static_cast<uint32_t>(tile[i + k + 2][tid]) << 16 | static_cast<uint32_t>(tile[i + k + 3][tid]) << 24;
+        };
+        if (len == kBlock && run_slot % 16 == 0 && pools.page_size % 16 == 0) {
+          *reinterpret_cast<uint4*>(to) = make_uint4(four(0), four(4), four(8), four(12));
+        } else {
+          for (int k = 0; k < len;) {
+            if ((run_slot + k) % 4 == 0 && k + 4 <= len && pools.page_size % 4 == 0) {
+              *reinterpret_cast<uint32_t*>(to + k) = four(k);
+              k += 4;
+            } else {
+              to[k] = tile[i + k][tid];
+              ++k;
+            }
+          }
+        }
       }
+      i += len;
+    }
+    return;
+  }
+
+  // ---- queries and keys of a token
+  const int t = blockIdx.x - value_groups, pos = a.positions[t];
+  const int lane = tid % LANES;
+  const bool on = lane * 8 < half;  // (a head of 96 elements has six of eight lanes)
+  const int items = (a.heads + (a.write_kv ? a.kv_heads : 0)) * LANES;
+  float x1[8], x2[8];
+  auto ask = [&](int item) {
+    if (item < items && on) {
+      fetch(t, item / LANES * dim + lane * 8, x1);
+      fetch(t, item / LANES * dim + half + lane * 8, x2);
+    }
+  };
+  ask(tid);  // travels while the cosines are formed
+  const int page =
+      a.write_kv ? e4m3_page(a.tables, a.table_stride, a.num_seqs, a.token_seq[t], pos, pools.page_size, pools.num_pages) : -1;
+  const int slot = page >= 0 ? pos % pools.page_size : 0;
+  for (int f = tid; f < half; f += kStoreThreads) turn_of(pos, a.inv_freq[f], a.magnitude, cs[f], sn[f]);
+  __syncthreads();
+  for (int item = tid; item < items; item += kStoreThreads) {
+    const int r = item / LANES;
+    float y1[8], y2[8];
+    uint32_t largest = 0;
+    if (on) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float c = cs[lane * 8 + e], s = sn[lane * 8 + e];
+        y1[e] = x1[e] * c - x2[e] * s;
+        y2[e] = x2[e] * c + x1[e] * s;
+      }
+      largest = max(largest_of(y1), largest_of(y2));
+    }
+    ask(item + kStoreThreads);
+    if (r < a.heads) {
+      if (!on) continue;
+      bf16* to = static_cast<bf16*>(a.q_out) + static_cast<size_t>(t) * a.q_ld + r * dim + lane * 8;
+      auto pack = [](const float (&y)[8]) {
+        return make_uint4(bf16_bits(y[0]) | static_cast<uint32_t>(bf16_bits(y[1])) << 16, bf16_bits(y[2]) | static_cast<uint32_t>(bf16_bits(y[3])) << 16,
+                          bf16_bits(y[4]) | static_cast<uint32_t>(bf16_bits(y[5])) << 16, bf16_bits(y[6]) | static_cast<uint32_t>(bf16_bits(y[7])) << 16);
+      };
+      *reinterpret_cast<uint4*>(to) = pack(y1);
+      *reinterpret_cast<uint4*>(to + half) = pack(y2);
       continue;
     }
 #pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) {
-      const uint32_t other = __shfl_xor(static_cast<int>(largest), off, kWave);
-      largest = other > largest ? other : largest;
-    }
+    for (int off = LANES / 2; off > 0; off >>= 1)
+      largest = max(largest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(largest), off, LANES)));
+    if (page < 0) continue;
     const int byte = e4m3_exponent_byte(largest);
+    const size_t where = pools.part(page, r - a.heads);
+    if (lane == 0) pools.scales[where * 2 * pools.page_size + slot] = static_cast<uint8_t>(byte);
+    if (!on) continue;
+    uint8_t* to = pools.k + where * pools.row_bytes();
     const float inverse = e4m3_inverse_unit(byte);
-    const int head = r - a.heads - (value ? a.kv_heads : 0);
-    const size_t part = pools.part(page, head), at = part * pools.row_bytes();
-    if (lane == 0) pools.scales[(part * 2 + (value ? 1 : 0)) * pools.page_size + slot] = static_cast<uint8_t>(byte);
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const int d = lane + i * kWave;
-      if (d >= dim) continue;
-      const uint8_t code = e4m3_code(x[i], inverse, largest);
-      if (value)
-        pools.v[at + static_cast<size_t>(d) * pools.page_size + slot] = code;
-      else
-        pools.k[at + key_offset(slot, d, pools.page_size, dim)] = code;
-    }
+    *reinterpret_cast<uint2*>(to + key_offset(slot, lane * 8, pools.page_size, dim)) = codes(y1, inverse, largest);
+    *reinterpret_cast<uint2*>(to + key_offset(slot, half + lane * 8, pools.page_size, dim)) = codes(y2, inverse, largest);
   }
 }
 
@@ -127,6 +344,96 @@ __global__ void __launch_bounds__(kStoreThreads)
     }
     k_out[out + i] = from_float<T>(k);
     v_out[out + i] = from_float<T>(v);
+  }
+}
+
+// The same for heads of a multiple of 32 elements: 16 neighbouring tokens of the call and one head a workgroup.  Keys go from 8-byte
+// pieces of a slab into 16-byte pieces of a row (of bfloat16); values come 16 tokens of an element at a time where the tokens fill a block
+// of 16, and turn in LDS.
+template <typename T>
+__device__ __forceinline__ void leave8(T* to, uint2 codes, float unit) {
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = e4m3_value((e < 4 ? codes.x : codes.y) >> (e % 4 * 8), unit);
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(to) =
+        make_uint4(bf16_bits(x[0]) | static_cast<uint32_t>(bf16_bits(x[1])) << 16, bf16_bits(x[2]) | static_cast<uint32_t>(bf16_bits(x[3])) << 16,
+                   bf16_bits(x[4]) | static_cast<uint32_t>(bf16_bits(x[5])) << 16, bf16_bits(x[6]) | static_cast<uint32_t>(bf16_bits(x[7])) << 16);
+  } else {
+    reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kStoreThreads)
+    read_blocks_e4m3_kernel(T* __restrict__ k_out, T* __restrict__ v_out, int n, const int32_t* __restrict__ positions,
+                            const int32_t* __restrict__ token_seq, const int32_t* __restrict__ tables, int table_stride, int num_seqs,
+                            E4m3Pools pools) {
+  __shared__ __attribute__((aligned(16))) uint8_t tile[kBlock][kMaxDim + 4];
+  __shared__ int pages[kBlock], slots[kBlock];
+  const int tid = threadIdx.x, dim = pools.head_dim, ps = pools.page_size;
+  const int head = blockIdx.x % pools.kv_heads, first = blockIdx.x / pools.kv_heads * kBlock;
+  const int mine = tid / 16, lane16 = tid % 16, t = first + mine, token = min(t, n - 1), pos = positions[token];
+  const int page = e4m3_page(tables, table_stride, num_seqs, token_seq[token], pos, ps, pools.num_pages);
+  const int slot = page >= 0 ? pos % ps : 0;
+  const size_t part = pools.part(page >= 0 ? page : 0, head);
+  if (lane16 == 0) pages[mine] = page, slots[mine] = slot;
+  // a token that is not there: codes of NaN
+  uint2 k_codes[2] = {make_uint2(kE4m3Nan, kE4m3Nan), make_uint2(kE4m3Nan, kE4m3Nan)};
+  int k_byte = 127, v_byte = 127;
+  if (page >= 0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = (lane16 + 16 * i) * 8;
+      if (d < dim) k_codes[i] = *reinterpret_cast<const uint2*>(pools.k + part * pools.row_bytes() + key_offset(slot, d, ps, dim));
+    }
+    k_byte = pools.scales[part * 2 * ps + slot];
+    v_byte = pools.scales[(part * 2 + 1) * ps + slot];
+  }
+  __syncthreads();
+  if (tid < dim) {
+    for (int i = 0; i < kBlock;) {
+      const int run_page = __builtin_amdgcn_readfirstlane(pages[i]), run_slot = __builtin_amdgcn_readfirstlane(slots[i]);
+      int len = 1;
+      while (i + len < kBlock && pages[i + len] == run_page && slots[i + len] == run_slot + len) ++len;
+      if (run_page < 0) {
+        tile[i][tid] = 0x7f;
+        ++i;
+        continue;
+      }
+      const uint8_t* from = pools.v + pools.part(run_page, head) * pools.row_bytes() + static_cast<size_t>(tid) * ps + run_slot;
+      auto put = [&](int k, uint32_t w) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) tile[i + k + b][tid] = static_cast<uint8_t>(w >> (8 * b));
+      };
+      if (len == kBlock && run_slot % 16 == 0 && ps % 16 == 0) {
+        const uint4 w = *reinterpret_cast<const uint4*>(from);
+        put(0, w.x), put(4, w.y), put(8, w.z), put(12, w.w);
+      } else {
+        for (int k = 0; k < len;) {
+          if ((run_slot + k) % 4 == 0 && k + 4 <= len && ps % 4 == 0) {
+            put(k, *reinterpret_cast<const uint32_t*>(from + k));
+            k += 4;
+          } else {
+            tile[i + k][tid] = from[k];
+            ++k;
+          }
+        }
+      }
+      i += len;
+    }
+  }
+  __syncthreads();
+  if (t >= n) return;
+  const size_t out = (static_cast<size_t>(t) * pools.kv_heads + head) * dim;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int d = (lane16 + 16 * i) * 8;
+    if (d >= dim) continue;
+    leave8(k_out + out + d, k_codes[i], e4m3_unit(k_byte));
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&tile[mine][d]);
+    leave8(v_out + out + d, make_uint2(w[0], w[1]), e4m3_unit(v_byte));
   }
 }
 
@@ -162,10 +469,19 @@ extern "C" int shk_rope_kv_store_e4m3(const void* qkv, int dtype, int n, int hea
   const E4m3Pools pools{static_cast<uint8_t*>(k_pool), static_cast<uint8_t*>(v_pool), static_cast<uint8_t*>(scales), page_size,
                         num_pages, kv_heads, head_dim};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == kF32)
-    store_e4m3_kernel<float><<<n, kStoreThreads, 0, s>>>(a, pools);
-  else
-    store_e4m3_kernel<bf16><<<n, kStoreThreads, 0, s>>>(a, pools);
+  if (n >= kManyTokens && dtype == kBF16 && rot_dim == head_dim && head_dim % 32 == 0 && !pairing && !v_from_k && q_ld % 8 == 0 &&
+      reinterpret_cast<uintptr_t>(splits ? static_cast<const void*>(parts) : qkv) % 16 == 0 && reinterpret_cast<uintptr_t>(q_out) % 16 == 0) {
+    const unsigned value_groups = write_kv ? static_cast<unsigned>((n + kBlock - 1) / kBlock * kv_heads) : 0;
+    const auto kernel = head_dim <= 64 ? store_many_e4m3_kernel<4> : head_dim <= 128 ? store_many_e4m3_kernel<8> : store_many_e4m3_kernel<16>;
+    kernel<<<value_groups + n, kStoreThreads, 0, s>>>(a, pools, value_groups);
+  } else {
+    const int row_groups = (heads + (write_kv ? 2 * kv_heads : 0) + kStoreWaves - 1) / kStoreWaves;
+    SHK_REQUIRE(static_cast<long long>(n) * row_groups < (1LL << 31), "rope_kv_store_e4m3: too many tokens: %d", n);
+    if (dtype == kF32)
+      store_e4m3_kernel<float><<<n * row_groups, kStoreThreads, 0, s>>>(a, pools, row_groups);
+    else
+      store_e4m3_kernel<bf16><<<n * row_groups, kStoreThreads, 0, s>>>(a, pools, row_groups);
+  }
   SHK_LAUNCH_CHECK("rope_kv_store_e4m3");
   return 0;
 }
@@ -184,12 +500,23 @@ extern "C" int shk_kv_read_e4m3(void* k_out, void* v_out, int dtype, int n, int 
   const E4m3Pools pools{static_cast<uint8_t*>(const_cast<void*>(k_pool)), static_cast<uint8_t*>(const_cast<void*>(v_pool)),
                         static_cast<uint8_t*>(const_cast<void*>(scales)), page_size, num_pages, kv_heads, head_dim};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == kF32)
-    read_e4m3_kernel<float><<<n, kStoreThreads, 0, s>>>(static_cast<float*>(k_out), static_cast<float*>(v_out), positions, token_seq,
-                                                        tables, table_stride, num_seqs, pools);
-  else
-    read_e4m3_kernel<bf16><<<n, kStoreThreads, 0, s>>>(static_cast<bf16*>(k_out), static_cast<bf16*>(v_out), positions, token_seq,
-                                                       tables, table_stride, num_seqs, pools);
+  const bool blocks = head_dim % 32 == 0 && reinterpret_cast<uintptr_t>(k_out) % 16 == 0 && reinterpret_cast<uintptr_t>(v_out) % 16 == 0;
+  const int grid = blocks ? (n + kBlock - 1) / kBlock * kv_heads : n;
+  if (dtype == kF32) {
+    if (blocks)
+      read_blocks_e4m3_kernel<float><<<grid, kStoreThreads, 0, s>>>(static_cast<float*>(k_out), static_cast<float*>(v_out), n, positions,
+                                                                    token_seq, tables, table_stride, num_seqs, pools);
+    else
+      read_e4m3_kernel<float><<<grid, kStoreThreads, 0, s>>>(static_cast<float*>(k_out), static_cast<float*>(v_out), positions, token_seq,
+                                                             tables, table_stride, num_seqs, pools);
+  } else {
+    if (blocks)
+      read_blocks_e4m3_kernel<bf16><<<grid, kStoreThreads, 0, s>>>(static_cast<bf16*>(k_out), static_cast<bf16*>(v_out), n, positions,
+                                                                   token_seq, tables, table_stride, num_seqs, pools);
+    else
+      read_e4m3_kernel<bf16><<<grid, kStoreThreads, 0, s>>>(static_cast<bf16*>(k_out), static_cast<bf16*>(v_out), positions, token_seq,
+                                                            tables, table_stride, num_seqs, pools);
+  }
   SHK_LAUNCH_CHECK("kv_read_e4m3");
   return 0;
 }

@@ -156,23 +156,34 @@ def decode_streams(num_seqs: int, kv_heads: int, head_dim: int, max_ctx: int, wi
 
 def e4m3_decode_splits(num_seqs: int, heads: int, kv_heads: int, head_dim: int, max_ctx: int) -> int:
     """Workgroups that share a single token's keys in a quantised cache: as many as put one on every compute unit, each with at
-    least KEYS_PER_WORKGROUP keys for its four wavefronts.  Rounded up as in decode_splits()."""
+    least KEYS_PER_WORKGROUP keys for its four wavefronts; up to 512 keys none, where a second launch takes longer than the
+    wavefronts' second chunk (one sequence of 333, 14 heads of 64 over 2: 6.2 us, 7.6 in two).  28 heads of 128 over 4, us unshared / so:
+    one sequence of 2,000 14.4 / 9.0, 8 of 2,060 16.3 / 11.4; 40 over 8, 8 of 16,000 93 / 52; shares beyond a workgroup a unit lose what
+    joining them costs (64 sequences of 61 to 4,000 36 unshared, 38 in 4).  Rounded up as in decode_splits()."""
+    keys = _pow2(max_ctx, KEYS_PER_WORKGROUP)
+    if keys <= 2 * KEYS_PER_WORKGROUP:
+        return 1
     tiles = kv_heads * -(-heads // (16 * kv_heads))
     want = -(-compute_units() // (_pow2(num_seqs) * tiles))
-    most = max(1, _pow2(max_ctx, KEYS_PER_WORKGROUP) // KEYS_PER_WORKGROUP)
-    return max(1, min(want, most, MAX_KEY_SPLITS))
+    return max(1, min(want, keys // KEYS_PER_WORKGROUP, MAX_KEY_SPLITS))
+
+
+E4M3_ROWS = 128  # rows (queries times heads of a key/value head) a workgroup of the quantised cache's prompt kernel
+E4M3_SHARE_KEYS = 128  # a turn of its two teams of wavefronts
 
 
 def e4m3_portion_splits(q_lens, starts, heads: int, kv_heads: int, head_dim: int, reach: int) -> int:
     """Workgroups that share the keys of a run of queries in a quantised cache (`reach`: the most keys that a query reads): as many
-    as bring the launch to the number of compute units, each worth KEYS_PER_WORKGROUP keys or more on average."""
-    queries = max(1, 128 // (heads // kv_heads))
-    runs, keys, total = 0, 0, 0
+    as the launch leaves compute units for, each worth E4M3_SHARE_KEYS keys or more on average.  us unshared / so: 4 times 17 tokens at
+    700 to 1,900 of 14 heads of 64 over 2 27.7 / 14 (18 in 3), 8 tokens at 2,000 of 28 of 128 over 4 35 / 14.6, 512 at 16,000 224 / 145 in 2; in
+    twice as many 149, for the float32 results of a prompt's shares are large (2,048 at 0: 57 unshared, 92 in 2)."""
+    queries = max(1, E4M3_ROWS // (heads // kv_heads))
+    runs = keys = total = 0
     for n, start in zip(q_lens, starts):
         runs += -(-n // queries)
         keys += n * min(start + n // 2, reach)
         total += n
-    return max(1, min(compute_units() // max(1, runs * kv_heads), keys // max(1, total) // KEYS_PER_WORKGROUP, MAX_KEY_SPLITS))
+    return max(1, min(compute_units() // max(1, runs * kv_heads), keys // max(1, total) // E4M3_SHARE_KEYS, MAX_KEY_SPLITS))
 
 
 @dataclass
