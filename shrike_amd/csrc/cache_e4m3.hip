@@ -142,6 +142,16 @@ __global__ void __launch_bounds__(kStoreThreads) store_e4m3_kernel(StoreArgs a, 
   }
 }
 
+// The 4 x 4 bytes whose rows are w, turned.
+__device__ __forceinline__ void turn4(uint32_t (&w)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+  const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
 // Many tokens of bfloat16 rows that turn whole, (i, i + head_dim / 2) together, head_dim a multiple of 32.  Queries and keys: a
 // workgroup per token, kLanes lanes a head with eight pairs each (16-byte loads, 8-byte pieces of codes) and a table of cosines.
 // Values: 16 neighbouring tokens of a step and one key/value head a workgroup; their codes turn in LDS, so that what lies side by side in a page
@@ -234,6 +244,20 @@ __global__ void __launch_bounds__(kStoreThreads) store_many_e4m3_kernel(StoreArg
     int* pages = reinterpret_cast<int*>(cs);  // of the 16 tokens, then their slots
     if (lane16 == 0) pages[mine] = page, pages[kBlock + mine] = slot;
     __syncthreads();
+    if (__syncthreads_and(page >= 0 && page == pages[0] && slot == mine + pages[kBlock] && pages[kBlock] % 16 == 0 && pools.page_size % 16 == 0)) {
+      // a block of 16: four tokens (tid % 4) of four elements
+      if (tid < dim) {
+        const int d = tid / 4 * 4, k = tid % 4 * 4;
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = *reinterpret_cast<const uint32_t*>(&tile[k + e][d]);
+        turn4(w);
+        uint8_t* to = pools.v + pools.part(page, head) * pools.row_bytes() + slot - mine + k;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(to + static_cast<size_t>(d + e) * pools.page_size) = w[e];
+      }
+      return;
+    }
     if (tid >= dim) return;
     // runs of tokens that are neighbours in a page, the same for every thread
     for (int i = 0; i < kBlock;) {
@@ -246,17 +270,13 @@ __global__ void __launch_bounds__(kStoreThreads) store_many_e4m3_kernel(StoreArg
           return static_cast<uint32_t>(tile[i + k][tid]) | static_cast<uint32_t>(tile[i + k + 1][tid]) << 8 |
                  static_cast<uint32_t>(tile[i + k + 2][tid]) << 16 | static_cast<uint32_t>(tile[i + k + 3][tid]) << 24;
         };
-        if (len == kBlock && run_slot % 16 == 0 && pools.page_size % 16 == 0) {
-          *reinterpret_cast<uint4*>(to) = make_uint4(four(0), four(4), four(8), four(12));
-        } else {
-          for (int k = 0; k < len;) {
-            if ((run_slot + k) % 4 == 0 && k + 4 <= len && pools.page_size % 4 == 0) {
-              *reinterpret_cast<uint32_t*>(to + k) = four(k);
-              k += 4;
-            } else {
-              to[k] = tile[i + k][tid];
-              ++k;
-            }
+        for (int k = 0; k < len;) {
+          if ((run_slot + k) % 4 == 0 && k + 4 <= len && pools.page_size % 4 == 0) {
+            *reinterpret_cast<uint32_t*>(to + k) = four(k);
+            k += 4;
+          } else {
+            to[k] = tile[i + k][tid];
+            ++k;
           }
         }
       }
@@ -348,8 +368,12 @@ __global__ void __launch_bounds__(kStoreThreads)
 }
 
 // The same for heads of a multiple of 32 elements: 16 neighbouring tokens of the call and one head a workgroup.  Keys go from 8-byte
-// pieces of a slab into 16-byte pieces of a row (of bfloat16); values come 16 tokens of an element at a time where the tokens fill a block
-// of 16, and turn in LDS.
+// pieces of a slab into 16-byte pieces of a row (of bfloat16).  Values of tokens that fill a block of 16 come in whole lines and turn
+// on their way, four by four bytes in registers and the rest through LDS; those of other tokens byte by byte, all at once: what a few
+// scattered tokens cost is one load's way.  128,000 tokens of 4 heads of 128 131 us with the values' bytes put into LDS one by
+// one, a thread an element.
+constexpr int kReadThreads = 128;
+
 template <typename T>
 __device__ __forceinline__ void leave8(T* to, uint2 codes, float unit) {
   float x[8];
@@ -366,74 +390,78 @@ __device__ __forceinline__ void leave8(T* to, uint2 codes, float unit) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kStoreThreads)
+__global__ void __launch_bounds__(kReadThreads)
     read_blocks_e4m3_kernel(T* __restrict__ k_out, T* __restrict__ v_out, int n, const int32_t* __restrict__ positions,
                             const int32_t* __restrict__ token_seq, const int32_t* __restrict__ tables, int table_stride, int num_seqs,
                             E4m3Pools pools) {
+  constexpr int kLanes = kReadThreads / kBlock, kRounds = kMaxDim / 8 / kLanes;  // of a token; of eight elements a lane
   __shared__ __attribute__((aligned(16))) uint8_t tile[kBlock][kMaxDim + 4];
-  __shared__ int pages[kBlock], slots[kBlock];
   const int tid = threadIdx.x, dim = pools.head_dim, ps = pools.page_size;
   const int head = blockIdx.x % pools.kv_heads, first = blockIdx.x / pools.kv_heads * kBlock;
-  const int mine = tid / 16, lane16 = tid % 16, t = first + mine, token = min(t, n - 1), pos = positions[token];
-  const int page = e4m3_page(tables, table_stride, num_seqs, token_seq[token], pos, ps, pools.num_pages);
+  const int mine = tid / kLanes, lane = tid % kLanes, t = first + mine, token = min(t, n - 1);
+  const int pos = positions[token], seq = token_seq[token];
+  // whether the tokens are a block of 16 of one page, in order: every wavefront looks at all of them
+  const int other = first + tid % kBlock, pos0 = positions[first];
+  const bool next = other < n && token_seq[min(other, n - 1)] == token_seq[first] && positions[min(other, n - 1)] == pos0 + tid % kBlock;
+  const bool in_order = __builtin_amdgcn_ballot_w64(next) == ~0ull && pos0 % kBlock == 0 && ps % kBlock == 0;
+  const int page = e4m3_page(tables, table_stride, num_seqs, seq, pos, ps, pools.num_pages);
   const int slot = page >= 0 ? pos % ps : 0;
-  const size_t part = pools.part(page >= 0 ? page : 0, head);
-  if (lane16 == 0) pages[mine] = page, slots[mine] = slot;
+  const size_t part = pools.part(page >= 0 ? page : 0, head), base = part * pools.row_bytes();
+  const bool whole = in_order && page >= 0;  // (one page: the same for every thread)
   // a token that is not there: codes of NaN
-  uint2 k_codes[2] = {make_uint2(kE4m3Nan, kE4m3Nan), make_uint2(kE4m3Nan, kE4m3Nan)};
+  uint2 k_codes[kRounds], v_codes[kRounds];
   int k_byte = 127, v_byte = 127;
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) k_codes[i] = v_codes[i] = make_uint2(kE4m3Nan, kE4m3Nan);
   if (page >= 0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int d = (lane16 + 16 * i) * 8;
-      if (d < dim) k_codes[i] = *reinterpret_cast<const uint2*>(pools.k + part * pools.row_bytes() + key_offset(slot, d, ps, dim));
+    for (int i = 0; i < kRounds; ++i) {
+      const int d = (lane + kLanes * i) * 8;
+      if (d < dim) k_codes[i] = *reinterpret_cast<const uint2*>(pools.k + base + key_offset(slot, d, ps, dim));
     }
     k_byte = pools.scales[part * 2 * ps + slot];
     v_byte = pools.scales[(part * 2 + 1) * ps + slot];
   }
-  __syncthreads();
-  if (tid < dim) {
-    for (int i = 0; i < kBlock;) {
-      const int run_page = __builtin_amdgcn_readfirstlane(pages[i]), run_slot = __builtin_amdgcn_readfirstlane(slots[i]);
-      int len = 1;
-      while (i + len < kBlock && pages[i + len] == run_page && slots[i + len] == run_slot + len) ++len;
-      if (run_page < 0) {
-        tile[i][tid] = 0x7f;
-        ++i;
-        continue;
-      }
-      const uint8_t* from = pools.v + pools.part(run_page, head) * pools.row_bytes() + static_cast<size_t>(tid) * ps + run_slot;
-      auto put = [&](int k, uint32_t w) {
+  if (whole) {
+    const uint8_t* from = pools.v + base + slot - mine;
+    // four tokens (tid % 4) of four elements
+    for (int at = tid; at < dim; at += kReadThreads) {
+      const int d = at / 4 * 4, k = at % 4 * 4;
+      uint32_t w[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) tile[i + k + b][tid] = static_cast<uint8_t>(w >> (8 * b));
-      };
-      if (len == kBlock && run_slot % 16 == 0 && ps % 16 == 0) {
-        const uint4 w = *reinterpret_cast<const uint4*>(from);
-        put(0, w.x), put(4, w.y), put(8, w.z), put(12, w.w);
-      } else {
-        for (int k = 0; k < len;) {
-          if ((run_slot + k) % 4 == 0 && k + 4 <= len && ps % 4 == 0) {
-            put(k, *reinterpret_cast<const uint32_t*>(from + k));
-            k += 4;
-          } else {
-            tile[i + k][tid] = from[k];
-            ++k;
-          }
-        }
-      }
-      i += len;
+      for (int e = 0; e < 4; ++e) w[e] = *reinterpret_cast<const uint32_t*>(from + static_cast<size_t>(d + e) * ps + k);
+      turn4(w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(&tile[k + e][d]) = w[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int d = (lane + kLanes * i) * 8;
+      if (d >= dim) continue;
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&tile[mine][d]);
+      v_codes[i] = make_uint2(w[0], w[1]);
+    }
+  } else if (page >= 0) {
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int d = (lane + kLanes * i) * 8;
+      if (d >= dim) continue;
+      const uint8_t* from = pools.v + base + static_cast<size_t>(d) * ps + slot;
+      uint32_t w[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e / 4] |= static_cast<uint32_t>(from[static_cast<size_t>(e) * ps]) << (e % 4 * 8);
+      v_codes[i] = make_uint2(w[0], w[1]);
     }
   }
-  __syncthreads();
   if (t >= n) return;
   const size_t out = (static_cast<size_t>(t) * pools.kv_heads + head) * dim;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int d = (lane16 + 16 * i) * 8;
+  for (int i = 0; i < kRounds; ++i) {
+    const int d = (lane + kLanes * i) * 8;
     if (d >= dim) continue;
     leave8(k_out + out + d, k_codes[i], e4m3_unit(k_byte));
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&tile[mine][d]);
-    leave8(v_out + out + d, make_uint2(w[0], w[1]), e4m3_unit(v_byte));
+    leave8(v_out + out + d, v_codes[i], e4m3_unit(v_byte));
   }
 }
 
@@ -504,14 +532,14 @@ extern "C" int shk_kv_read_e4m3(void* k_out, void* v_out, int dtype, int n, int 
   const int grid = blocks ? (n + kBlock - 1) / kBlock * kv_heads : n;
   if (dtype == kF32) {
     if (blocks)
-      read_blocks_e4m3_kernel<float><<<grid, kStoreThreads, 0, s>>>(static_cast<float*>(k_out), static_cast<float*>(v_out), n, positions,
+      read_blocks_e4m3_kernel<float><<<grid, kReadThreads, 0, s>>>(static_cast<float*>(k_out), static_cast<float*>(v_out), n, positions,
                                                                     token_seq, tables, table_stride, num_seqs, pools);
     else
       read_e4m3_kernel<float><<<grid, kStoreThreads, 0, s>>>(static_cast<float*>(k_out), static_cast<float*>(v_out), positions, token_seq,
                                                              tables, table_stride, num_seqs, pools);
   } else {
     if (blocks)
-      read_blocks_e4m3_kernel<bf16><<<grid, kStoreThreads, 0, s>>>(static_cast<bf16*>(k_out), static_cast<bf16*>(v_out), n, positions,
+      read_blocks_e4m3_kernel<bf16><<<grid, kReadThreads, 0, s>>>(static_cast<bf16*>(k_out), static_cast<bf16*>(v_out), n, positions,
                                                                    token_seq, tables, table_stride, num_seqs, pools);
     else
       read_e4m3_kernel<bf16><<<grid, kStoreThreads, 0, s>>>(static_cast<bf16*>(k_out), static_cast<bf16*>(v_out), positions, token_seq,

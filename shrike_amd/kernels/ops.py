@@ -808,10 +808,12 @@ def e4m3_scales_shape(pages: int, kv_heads: int, page_size: int) -> tuple:
 
 
 def _e4m3_cache(who, kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size) -> tuple:
-    """Arguments (tables, table_stride, num_seqs, pools, scales, page_size, num_pages) of a launcher, checked."""
+    """Arguments (tables, table_stride, num_seqs, pools, scales, page_size, num_pages) of a launcher, checked.  (A call of these functions is
+    often shorter on the device than here, hence few calls.)"""
+    if k_pool.dtype is not E4M3 or v_pool.dtype is not E4M3 or scales.dtype is not torch.uint8 or tables.dtype is not torch.int32:
+        raise KernelError(f"{who}: pools must be float8_e4m3fn, scales uint8 and tables int32, got {k_pool.dtype}, {v_pool.dtype}, "
+                          f"{scales.dtype} and {tables.dtype}")
     pages = k_pool.shape[0]
-    if k_pool.dtype != E4M3 or v_pool.dtype != E4M3 or scales.dtype != torch.uint8:
-        raise KernelError(f"{who}: pools must be float8_e4m3fn and scales uint8, got {k_pool.dtype}, {v_pool.dtype}, {scales.dtype}")
     if k_pool.shape != key_pool_shape(pages, kv_heads, page_size, head_dim):
         raise KernelError(f"{who}: key pool must be {list(key_pool_shape('pages', kv_heads, page_size, head_dim))}, "
                           f"got {tuple(k_pool.shape)}")
@@ -820,18 +822,23 @@ def _e4m3_cache(who, kv_heads, head_dim, tables, k_pool, v_pool, scales, page_si
                           f"[{pages}, {kv_heads}, 2, {page_size}], got {tuple(v_pool.shape)} and {tuple(scales.shape)}")
     if not (k_pool.is_contiguous() and v_pool.is_contiguous() and scales.is_contiguous() and tables.is_contiguous()):
         raise KernelError(f"{who}: pools, scales and tables must be contiguous")
-    if tables.dim() != 2:
+    size = tables.shape
+    if len(size) != 2:
         raise KernelError(f"{who}: tables must be [sequences, blocks]")
-    if k_pool.data_ptr() % 16 or v_pool.data_ptr() % 16 or scales.data_ptr() % 16:
+    if not (k_pool.is_cuda and v_pool.is_cuda and scales.is_cuda and tables.is_cuda):
+        raise KernelError(f"{who}: expected device tensors (there is no CPU path)")
+    k, v, e = k_pool.data_ptr(), v_pool.data_ptr(), scales.data_ptr()
+    if (k | v | e) & 15:
         raise KernelError(f"{who}: pools and scales must be 16-byte aligned")
-    return (_dev(tables, "tables", torch.int32), tables.shape[1], tables.shape[0], _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool"),
-            _dev(scales, "scales"), page_size, pages)
+    return (tables.data_ptr(), size[1], size[0], k, v, e, page_size, pages)
 
 
-def _step_rows(who, n, *arrays) -> None:
-    for a in arrays:
-        if a.dim() != 1 or a.shape[0] < n or not a.is_contiguous():
-            raise KernelError(f"{who}: the call has {n} rows, and positions and token_seq must be contiguous with one number for each")
+def _step_rows(who, n, a) -> int:
+    """Address of an int32 array of the step with one number for each of n rows, checked."""
+    if a.dtype is not torch.int32 or not a.is_cuda or a.dim() != 1 or a.shape[0] < n or not a.is_contiguous():
+        raise KernelError(f"{who}: the call has {n} rows, and positions, token_seq, cu_q and ctx_lens must be contiguous int32 on the device "
+                          "with one number for each")
+    return a.data_ptr()
 
 
 def rope_kv_store_e4m3(qkv, heads, kv_heads, head_dim, rot_dim, inv_freq, positions, token_seq, tables, k_pool, v_pool, scales,
@@ -863,13 +870,10 @@ def rope_kv_store_e4m3(qkv, heads, kv_heads, head_dim, rot_dim, inv_freq, positi
     cache = (None, 0, 0, None, None, None, page_size, 0)
     if write_kv:
         cache = _e4m3_cache("rope_kv_store_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size)
-        _step_rows("rope_kv_store_e4m3", n, positions, token_seq)
-    else:
-        _step_rows("rope_kv_store_e4m3", n, positions)
     check(load().shk_rope_kv_store_e4m3(
         _dev(qkv, "qkv"), dtype_code(qkv.dtype), n, heads, kv_heads, head_dim, rot_dim,
-        _dev(inv_freq, "inv_freq", torch.float32) if rot_dim else None, _dev(positions, "positions", torch.int32),
-        _dev(token_seq, "token_seq", torch.int32) if write_kv else None, *cache, int(bool(write_kv)),
+        _dev(inv_freq, "inv_freq", torch.float32) if rot_dim else None, _step_rows("rope_kv_store_e4m3", n, positions),
+        _step_rows("rope_kv_store_e4m3", n, token_seq) if write_kv else None, *cache, int(bool(write_kv)),
         None if parts is None else _dev(parts, "parts"), splits, None if bias is None else _dev(bias, "bias", torch.float32),
         int(bool(adjacent_pairs)), int(bool(values_from_keys)), float(magnitude), _dev(q_out, "q_out"), q_out.stride(0), _stream()))
 
@@ -881,10 +885,9 @@ def kv_read_e4m3(k_out, v_out, kv_heads, head_dim, positions, token_seq, tables,
     if k_out.shape != (n, kv_heads * head_dim) or v_out.shape != k_out.shape or v_out.dtype != k_out.dtype \
             or not (k_out.is_contiguous() and v_out.is_contiguous()):
         raise KernelError("kv_read_e4m3: k_out and v_out must be contiguous [n, kv_heads * head_dim] of one dtype")
-    _step_rows("kv_read_e4m3", n, positions, token_seq)
     check(load().shk_kv_read_e4m3(
         _dev(k_out, "k_out"), _dev(v_out, "v_out"), dtype_code(k_out.dtype), n, kv_heads, head_dim,
-        _dev(positions, "positions", torch.int32), _dev(token_seq, "token_seq", torch.int32),
+        _step_rows("kv_read_e4m3", n, positions), _step_rows("kv_read_e4m3", n, token_seq),
         *_e4m3_cache("kv_read_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size), _stream()))
 
 
@@ -895,10 +898,9 @@ def attention_e4m3(q, out, heads, kv_heads, head_dim, positions, token_seq, tabl
     n = q.shape[0]
     if q.shape[1] < heads * head_dim or out.shape != (n, heads * head_dim) or not out.is_contiguous() or out.dtype != q.dtype:
         raise KernelError("attention_e4m3: out must be contiguous [n, heads * head_dim] of q's dtype, q at least as wide")
-    _step_rows("attention_e4m3", n, positions, token_seq)
     check(load().shk_attention_e4m3(
         _dev(q, "q"), q.stride(0), _dev(out, "out"), dtype_code(q.dtype), n, heads, kv_heads, head_dim,
-        _dev(positions, "positions", torch.int32), _dev(token_seq, "token_seq", torch.int32),
+        _step_rows("attention_e4m3", n, positions), _step_rows("attention_e4m3", n, token_seq),
         *_e4m3_cache("attention_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size), int(window or 0),
         int(chunk or 0), float(scale), _stream()))
 
@@ -930,9 +932,9 @@ def attention_decode_e4m3(q, out, num_seqs, heads, kv_heads, head_dim, positions
     scratch = _e4m3_rows("attention_decode_e4m3", q, out, heads, head_dim, partial, num_seqs, nsplit)
     if q.shape[0] < num_seqs or out.shape[0] < num_seqs:
         raise KernelError("attention_decode_e4m3: fewer rows than sequences")
-    _step_rows("attention_decode_e4m3", num_seqs, positions)
     check(load().shk_attention_decode_e4m3(
-        _dev(q, "q"), q.stride(0), _dev(out, "out"), num_seqs, heads, kv_heads, head_dim, _dev(positions, "positions", torch.int32),
+        _dev(q, "q"), q.stride(0), _dev(out, "out"), num_seqs, heads, kv_heads, head_dim,
+        _step_rows("attention_decode_e4m3", num_seqs, positions),
         *_e4m3_cache("attention_decode_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size), int(window or 0),
         int(chunk or 0), float(scale), scratch, nsplit, _stream()))
 
@@ -947,11 +949,10 @@ def attention_prefill_e4m3(q, out, first_seq, num_seqs, heads, kv_heads, head_di
     scratch = _e4m3_rows("attention_prefill_e4m3", q, out, heads, head_dim, partial, n - first_seq, nsplit)
     if out.shape[0] != n:
         raise KernelError("attention_prefill_e4m3: out must have a row for each of q's")
-    _step_rows("attention_prefill_e4m3", first_seq + num_seqs, ctx_lens)
-    _step_rows("attention_prefill_e4m3", first_seq + num_seqs + 1, cu_q)
     check(load().shk_attention_prefill_e4m3(
-        _dev(q, "q"), q.stride(0), _dev(out, "out"), n, first_seq, num_seqs, heads, kv_heads, head_dim, _dev(cu_q, "cu_q", torch.int32),
-        _dev(ctx_lens, "ctx_lens", torch.int32),
+        _dev(q, "q"), q.stride(0), _dev(out, "out"), n, first_seq, num_seqs, heads, kv_heads, head_dim,
+        _step_rows("attention_prefill_e4m3", first_seq + num_seqs + 1, cu_q),
+        _step_rows("attention_prefill_e4m3", first_seq + num_seqs, ctx_lens),
         *_e4m3_cache("attention_prefill_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size), int(window or 0),
         int(chunk or 0), float(scale), scratch, nsplit, _stream()))
 

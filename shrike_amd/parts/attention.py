@@ -159,31 +159,29 @@ def e4m3_decode_splits(num_seqs: int, heads: int, kv_heads: int, head_dim: int, 
     least KEYS_PER_WORKGROUP keys for its four wavefronts; up to 512 keys none, where a second launch takes longer than the
     wavefronts' second chunk (one sequence of 333, 14 heads of 64 over 2: 6.2 us, 7.6 in two).  28 heads of 128 over 4, us unshared / so:
     one sequence of 2,000 14.4 / 9.0, 8 of 2,060 16.3 / 11.4; 40 over 8, 8 of 16,000 93 / 52; shares beyond a workgroup a unit lose what
-    joining them costs (64 sequences of 61 to 4,000 36 unshared, 38 in 4).  Rounded up as in decode_splits()."""
-    keys = _pow2(max_ctx, KEYS_PER_WORKGROUP)
-    if keys <= 2 * KEYS_PER_WORKGROUP:
+    joining them costs (64 sequences of 61 to 4,000 36 unshared, 38 in 4).  The batch is rounded up to a power of two, as it is padded
+    for graphs; so that a graph serves more than one length, prepare() rounds the longest context too."""
+    if max_ctx <= 2 * KEYS_PER_WORKGROUP:
         return 1
     tiles = kv_heads * -(-heads // (16 * kv_heads))
     want = -(-compute_units() // (_pow2(num_seqs) * tiles))
-    return max(1, min(want, keys // KEYS_PER_WORKGROUP, MAX_KEY_SPLITS))
+    return max(1, min(want, -(-max_ctx // KEYS_PER_WORKGROUP), MAX_KEY_SPLITS))
 
 
 E4M3_ROWS = 128  # rows (queries times heads of a key/value head) a workgroup of the quantised cache's prompt kernel
-E4M3_SHARE_KEYS = 128  # a turn of its two teams of wavefronts
 
 
 def e4m3_portion_splits(q_lens, starts, heads: int, kv_heads: int, head_dim: int, reach: int) -> int:
     """Workgroups that share the keys of a run of queries in a quantised cache (`reach`: the most keys that a query reads): as many
-    as the launch leaves compute units for, each worth E4M3_SHARE_KEYS keys or more on average.  us unshared / so: 4 times 17 tokens at
-    700 to 1,900 of 14 heads of 64 over 2 27.7 / 14 (18 in 3), 8 tokens at 2,000 of 28 of 128 over 4 35 / 14.6, 512 at 16,000 224 / 145 in 2; in
+    as the launch leaves compute units for, each worth KEYS_PER_WORKGROUP of the longest sequence's keys.  us unshared / so: 4 times 17
+    tokens at 700 to 1,900 of 14 heads of 64 over 2 27.7 / 13.6, 8 tokens at 2,000 of 28 of 128 over 4 35 / 15.3, 512 at 16,000 224 / 145 in 2; in
     twice as many 149, for the float32 results of a prompt's shares are large (2,048 at 0: 57 unshared, 92 in 2)."""
     queries = max(1, E4M3_ROWS // (heads // kv_heads))
-    runs = keys = total = 0
+    runs = longest = 0
     for n, start in zip(q_lens, starts):
         runs += -(-n // queries)
-        keys += n * min(start + n // 2, reach)
-        total += n
-    return max(1, min(compute_units() // max(1, runs * kv_heads), keys // max(1, total) // E4M3_SHARE_KEYS, MAX_KEY_SPLITS))
+        longest = max(longest, start + n)
+    return max(1, min(compute_units() // max(1, runs * kv_heads), -(-min(longest, reach) // KEYS_PER_WORKGROUP), MAX_KEY_SPLITS))
 
 
 @dataclass
@@ -535,7 +533,7 @@ class PagedAttention(Mixer):
             if plan.mfma:
                 reach = min(x for x in (s.window, s.chunk, 1 << 40) if x)
                 if shape.num_decode:
-                    plan.nsplit = e4m3_decode_splits(shape.num_decode, h, hkv, d, min(shape.max_decode_ctx, reach))
+                    plan.nsplit = e4m3_decode_splits(shape.num_decode, h, hkv, d, _pow2(min(shape.max_decode_ctx, reach), KEYS_PER_WORKGROUP))
                 if shape.num_seqs > shape.num_decode:
                     plan.portion_splits = e4m3_portion_splits(shape.q_lens[shape.num_decode:].tolist(),
                                                               shape.starts[shape.num_decode:].tolist(), h, hkv, d, reach)

@@ -125,9 +125,10 @@ def test_launch_plans(heads, kv):
     for seqs in (1, 2, 7, 64, 300):
         for ctx in (1, 63, 256, 257, 5000, 131072):
             n = e4m3_decode_splits(seqs, heads, kv, 128, ctx)
-            assert 1 <= n <= 64
-            # a batch that is padded to the next power of two, and a longer context up to the next one, take the same
-            assert n == e4m3_decode_splits(1 << (seqs - 1).bit_length(), heads, kv, 128, max(256, 1 << (ctx - 1).bit_length()))
+            assert 1 <= n <= min(64, -(-ctx // 256))
+            # a batch that is padded to the next power of two takes the same
+            assert n == e4m3_decode_splits(1 << (seqs - 1).bit_length(), heads, kv, 128, ctx)
     for lens, starts in (([2], [0]), ([512], [16000]), ([17] * 4, [700, 800, 900, 1900]), ([2048], [0]), ([1, 0, 30], [5, 0, 9])):
-        assert 1 <= e4m3_portion_splits(lens, starts, heads, kv, 128, 1 << 40) <= 64
+        longest = max(a + n for a, n in zip(starts, lens))
+        assert 1 <= e4m3_portion_splits(lens, starts, heads, kv, 128, 1 << 40) <= min(64, -(-longest // 256))
         assert e4m3_portion_splits(lens, starts, heads, kv, 128, 100) == 1  # a window of 100 keys is not shared
