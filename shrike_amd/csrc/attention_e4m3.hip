@@ -418,10 +418,10 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
   constexpr int KS = D / 16, DB = D / 32;
   constexpr int kSide = 64 * D * 2;         // bytes of a chunk's keys as bfloat16, and of its values
   constexpr int kPer = (D + kWave - 1) / kWave;  // pieces of 16 codes of a block's keys that a lane brings, and of its values
-  // a team's keys of two chunks and values of two; in the end the second team's results
+  // a team's keys of two chunks and values of two; in the end half of either team's results
   __shared__ u32x4 mem[TEAMS][4 * kSide / 16];
   __shared__ float units[TEAMS][2][64], ends[TEAMS][2][kPortionRows];  // (units: of the values)
-  static_assert(TEAMS == 1 || TEAMS * 4 * kSide >= kPortionRows * D * 4, "the second team's sums fit");
+  static_assert(TEAMS == 1 || TEAMS * 4 * kSide >= kPortionRows * D * 4, "half of either team's sums fit");
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int team = wave / 4, member = wave % 4;
   const int col = lane % 32, half = lane / 32;
@@ -429,14 +429,15 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
   const PageDiv pd{page_size, a.page_magic};
   const int z = blockIdx.x % a.nsplit, kvh = blockIdx.x / a.nsplit % a.kv_heads;
 
-  // ---- this workgroup's sequence and first query
-  int seq = -1, q0 = 0;
+  // ---- this workgroup's sequence and first query: lane i looks at sequence i, so that one round of loads finds everything
+  const int group = a.heads / a.kv_heads;
+  int seq = -1, q0 = 0, tok0 = 0, tok1 = 0, ctx = 0;
   {
     int left = blockIdx.x / (a.nsplit * a.kv_heads);
     for (int base = 0; base < a.num_seqs; base += kWave) {
-      const int i = base + lane;
-      int runs = 0;
-      if (i < a.num_seqs) runs = (a.cu_q[a.first_seq + i + 1] - a.cu_q[a.first_seq + i] + a.queries - 1) / a.queries;
+      const int i = a.first_seq + min(base + lane, a.num_seqs - 1);
+      const int from = a.cu_q[i], to = a.cu_q[i + 1], length = a.ctx_lens[i];
+      const int runs = base + lane < a.num_seqs && to > from ? (to - from + a.queries - 1) / a.queries : 0;
       int upto = runs;
 #pragma unroll
       for (int off = 1; off < kWave; off <<= 1) {
@@ -447,19 +448,19 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
       if (past) {
         const int at = __builtin_ctzll(past);
         seq = a.first_seq + base + at;
-        q0 = (__shfl(upto, at, kWave) - 1 - left) * a.queries;
+        q0 = (__builtin_amdgcn_readlane(upto, at) - 1 - left) * a.queries;
+        tok0 = __builtin_amdgcn_readlane(from, at);
+        tok1 = __builtin_amdgcn_readlane(to, at);
+        ctx = __builtin_amdgcn_readlane(length, at);
         break;
       }
-      left -= __shfl(upto, kWave - 1, kWave);
+      left -= __builtin_amdgcn_readlane(upto, kWave - 1);
     }
     if (seq < 0) return;  // (there are at most as many runs as workgroups)
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    q0 = __builtin_amdgcn_readfirstlane(q0);
   }
-  const int group = a.heads / a.kv_heads;
-  const int tok0 = a.cu_q[seq], tok1 = a.cu_q[seq + 1], q_len = min(tok1, a.n) - tok0;
+  const int q_len = min(tok1, a.n) - tok0;
   if (tok0 < a.first_seq || q0 >= q_len) return;  // (ranges that are not the rows' are a mistake of the caller's, never followed)
-  const int start = a.ctx_lens[seq] - (tok1 - tok0);  // position of the run's first token
+  const int start = ctx - (tok1 - tok0);  // position of the run's first token
   const int q_end = q0 + a.queries < q_len ? q0 + a.queries : q_len;
   const int32_t* table = a.tables + static_cast<size_t>(seq) * a.table_stride;
 
@@ -764,6 +765,7 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
     }
     if (chunk_of(turns - 1) < c_end) add_values((turns - 1) % 2);
     if (TEAMS == 2 && team == 0) __syncthreads();
+    __syncthreads();  // LDS is read no more
   }
 
   float total;
@@ -772,59 +774,61 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
     const auto halves = __builtin_amdgcn_permlane32_swap(b, b, false, false);
     total = bits_as_float(halves[0]) + bits_as_float(halves[1]);
   }
+  // ---- the teams' results become one: each hands over half of its sums and finishes the other half
+  constexpr int kParts = DB * 4, kMine = TEAMS == 2 ? kParts / 2 : kParts;  // of four elements of a lane's row
+  const int first_part = TEAMS == 2 ? team * kMine : 0;
+  f32x4 sums[kMine];
+  float mine_by = 1.f;
   if (TEAMS == 2) {
-    // ---- the teams' results become one
-    __syncthreads();
-    f32x4* sums = reinterpret_cast<f32x4*>(&mem[0][0]);
-    if (team == 1) {
+    f32x4* over = reinterpret_cast<f32x4*>(&mem[0][0]);  // [the team that takes them][member][part][lane]
+    if (!half) ends[team][0][row] = m, ends[team][1][row] = total;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          sums[(member * DB * 4 + db * 4 + g) * kWave + lane] = f32x4{o[db][g * 4], o[db][g * 4 + 1], o[db][g * 4 + 2], o[db][g * 4 + 3]};
-      if (!half) ends[1][0][row] = m, ends[1][1][row] = total;
+    for (int i = 0; i < kMine; ++i) {
+      // (the indices are known when this is compiled: a team's parts by a select)
+      const f32x4 lo = {o[i / 4][i % 4 * 4], o[i / 4][i % 4 * 4 + 1], o[i / 4][i % 4 * 4 + 2], o[i / 4][i % 4 * 4 + 3]};
+      const int k = i + kMine;
+      const f32x4 hi = {o[k / 4][k % 4 * 4], o[k / 4][k % 4 * 4 + 1], o[k / 4][k % 4 * 4 + 2], o[k / 4][k % 4 * 4 + 3]};
+      over[(((1 - team) * 4 + member) * kMine + i) * kWave + lane] = team ? lo : hi;
+      sums[i] = team ? hi : lo;
     }
     __syncthreads();
-    if (team == 1) return;
-    const float other = ends[1][0][row], top = fmaxf(m, other), ref = top == -INFINITY ? 0.f : top;
-    const float mine_by = __builtin_amdgcn_exp2f((m - ref) * scale2), other_by = __builtin_amdgcn_exp2f((other - ref) * scale2);
-    total = total * mine_by + ends[1][1][row] * other_by;
+    const float other = ends[1 - team][0][row], top = fmaxf(m, other), ref = top == -INFINITY ? 0.f : top;
+    mine_by = __builtin_amdgcn_exp2f((m - ref) * scale2);
+    const float other_by = __builtin_amdgcn_exp2f((other - ref) * scale2);
+    total = total * mine_by + ends[1 - team][1][row] * other_by;
     m = top;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+    for (int i = 0; i < kMine; ++i) {
+      const f32x4 x = over[((team * 4 + member) * kMine + i) * kWave + lane];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 x = sums[(member * DB * 4 + db * 4 + g) * kWave + lane];
+      for (int r = 0; r < 4; ++r) sums[i][r] = sums[i][r] * mine_by + x[r] * other_by;
+    }
+  } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[db][g * 4 + r] = o[db][g * 4 + r] * mine_by + x[r] * other_by;
-      }
+    for (int i = 0; i < kMine; ++i) sums[i] = f32x4{o[i / 4][i % 4 * 4], o[i / 4][i % 4 * 4 + 1], o[i / 4][i % 4 * 4 + 2], o[i / 4][i % 4 * 4 + 3]};
   }
   if (!mine) return;
+  // (part i of a row: elements i / 4 * 32 + i % 4 * 8 + 4 half .. + 3)
   if (a.nsplit > 1) {
     // a share's result, for merge_e4m3_kernel: O [row][share][D], then (maximum, sum) [row][share][2]
     const size_t rows = static_cast<size_t>(a.n - a.first_seq) * a.heads;
     const size_t at = static_cast<size_t>(tok0 + qi - a.first_seq) * a.heads + head;
-    float* dst = a.partial + (at * a.nsplit + z) * D + 4 * half;
+    float* dst = a.partial + (at * a.nsplit + z) * D + 4 * half + first_part * 8;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(dst + db * 32 + g * 8) = f32x4{o[db][g * 4], o[db][g * 4 + 1], o[db][g * 4 + 2], o[db][g * 4 + 3]};
-    if (!half)
+    for (int i = 0; i < kMine; ++i) *reinterpret_cast<f32x4*>(dst + i * 8) = sums[i];
+    if (!half && team == 0)
       *reinterpret_cast<float2*>(a.partial + rows * a.nsplit * D + (at * a.nsplit + z) * 2) = make_float2(m * scale2, total);
     return;
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;  // (a query that reads no key: zeros)
-  bf16* dst = a.out + (static_cast<size_t>(tok0 + qi) * a.heads + head) * D + 4 * half;
+  bf16* dst = a.out + (static_cast<size_t>(tok0 + qi) * a.heads + head) * D + 4 * half + first_part * 8;
 #pragma unroll
-  for (int db = 0; db < DB; ++db)
+  for (int i = 0; i < kMine; ++i) {
+    bf16x4 v;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      bf16x4 v;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = static_cast<__bf16>(o[db][g * 4 + r] * inv);
-      *reinterpret_cast<bf16x4*>(dst + db * 32 + g * 8) = v;
-    }
+    for (int r = 0; r < 4; ++r) v[r] = static_cast<__bf16>(sums[i][r] * inv);
+    *reinterpret_cast<bf16x4*>(dst + i * 8) = v;
+  }
 }
 
 }  // namespace shk

@@ -169,19 +169,24 @@ def e4m3_decode_splits(num_seqs: int, heads: int, kv_heads: int, head_dim: int, 
 
 
 E4M3_ROWS = 128  # rows (queries times heads of a key/value head) a workgroup of the quantised cache's prompt kernel
+E4M3_SHARE_KEYS = 128  # a turn of its two teams of wavefronts
 
 
 def e4m3_portion_splits(q_lens, starts, heads: int, kv_heads: int, head_dim: int, reach: int) -> int:
     """Workgroups that share the keys of a run of queries in a quantised cache (`reach`: the most keys that a query reads): as many
-    as the launch leaves compute units for, each worth KEYS_PER_WORKGROUP of the longest sequence's keys.  us unshared / so: 4 times 17
-    tokens at 700 to 1,900 of 14 heads of 64 over 2 27.7 / 13.6, 8 tokens at 2,000 of 28 of 128 over 4 35 / 15.3, 512 at 16,000 224 / 145 in 2; in
-    twice as many 149, for the float32 results of a prompt's shares are large (2,048 at 0: 57 unshared, 92 in 2)."""
+    as the launch leaves compute units for, each worth E4M3_SHARE_KEYS keys on average and KEYS_PER_WORKGROUP of the longest sequence's.
+    us unshared / so: 4 times 17 tokens at 700 to 1,900 of 14 heads of 64 over 2 27.7 / 13.6, 8 tokens at 2,000 of 28 of 128 over 4 35 /
+    15.3, 512 at 16,000 224 / 145 in 2; in twice as many 149, for the float32 results of a prompt's shares are large (2,048 at 0: 57
+    unshared, 92 in 2; two of 300 at 0, 16 over 16 15.5 and 21)."""
     queries = max(1, E4M3_ROWS // (heads // kv_heads))
-    runs = longest = 0
+    runs = longest = keys = total = 0
     for n, start in zip(q_lens, starts):
         runs += -(-n // queries)
         longest = max(longest, start + n)
-    return max(1, min(compute_units() // max(1, runs * kv_heads), -(-min(longest, reach) // KEYS_PER_WORKGROUP), MAX_KEY_SPLITS))
+        keys += n * min(start + n // 2, reach)
+        total += n
+    return max(1, min(compute_units() // max(1, runs * kv_heads), keys // max(1, total) // E4M3_SHARE_KEYS,
+                      -(-min(longest, reach) // KEYS_PER_WORKGROUP), MAX_KEY_SPLITS))
 
 
 @dataclass
