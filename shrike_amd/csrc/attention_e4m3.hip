@@ -390,8 +390,10 @@ __global__ void __launch_bounds__(kWave) merge_e4m3_kernel(const float* __restri
 // that both would want the same unit at the same time.  Their results are joined through LDS in the end.
 //
 // Codes come from the pages into registers a turn ahead and go to LDS as bfloat16 values, each of them converted once for the
-// team's rows; a wavefront brings one block of 16 keys of every chunk.  Keys get their power of two in the conversion; that of a value
-// joins its key's weight in float32, behind the sum of the weights and before they are rounded.
+// team's rows; a wavefront brings one block of 16 keys of every chunk.  Keys get their power of two in the conversion.  A value's, 2^c,
+// costs nothing per weight: a score begins as c / scale2 instead of 0, so that its weight comes out times 2^c, and the
+// denominator is a product of the same rounded weights with 2^-c, on the matrix units too.  c is bounded by 40 either way, so that
+// neither leaves the range of the types; what lies beyond is multiplied onto the codes (seldom, and exactly).
 //   keys    [block of 16][32 elements] units of 1 KiB, 64 bytes a key: piece c of 16 bytes of a key at place c ^ (key / 4),
 //   values  [block of 16][32 elements] units, 32 bytes an element: piece c at place c ^ (element / 8 % 2),
 // so that the lanes that LDS serves together meet no bank conflicts.  Row 8 a + 4 h + r of a score tile is key 16 (a / 2) + 8 h +
@@ -400,7 +402,8 @@ __global__ void __launch_bounds__(kWave) merge_e4m3_kernel(const float* __restri
 // The workgroups find their queries themselves, a sequence's last queries (which read the most keys) first, so a step needs no
 // lists from the host.
 constexpr int kPortionRows = 128;
-constexpr float kLargeSum = 1024.f;  // of a chunk's weights relative to the reference: it moves
+constexpr float kSlack = 10.f;  // log2 of the largest weight relative to the reference: beyond it moves
+constexpr int kMostUnit = 40;
 
 struct PortionArgs {
   const bf16* q;
@@ -420,7 +423,9 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
   constexpr int kPer = (D + kWave - 1) / kWave;  // pieces of 16 codes of a block's keys that a lane brings, and of its values
   // a team's keys of two chunks and values of two; in the end half of either team's results
   __shared__ u32x4 mem[TEAMS][4 * kSide / 16];
-  __shared__ float units[TEAMS][2][64], ends[TEAMS][2][kPortionRows];  // (units: of the values)
+  __shared__ __attribute__((aligned(16))) float begin[TEAMS][2][64];       // a chunk's c / scale2 by key
+  __shared__ __attribute__((aligned(16))) uint16_t undo[TEAMS][2][64];     // 2^-c as bfloat16
+  __shared__ float ends[TEAMS][2][kPortionRows];
   static_assert(TEAMS == 1 || TEAMS * 4 * kSide >= kPortionRows * D * 4, "half of either team's sums fit");
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int team = wave / 4, member = wave % 4;
@@ -483,14 +488,15 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
 #pragma unroll
     for (int st = 0; st < KS; ++st) qf[st] = *reinterpret_cast<const bf16x8*>(src + st * 16);
   }
-  float m = -INFINITY, l = 0.f;  // the weights' reference, of the unscaled scores; the lane's share of the sum
+  float m = -INFINITY, l = 0.f;  // the weights' reference, of the unscaled scores; their sum
   f32x16 o[DB];                  // element db * 32 + 8 g + 4 half + r of the row in register g * 4 + r
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
   const float scale2 = a.scale * 1.4426950408889634f;
-  float shift = 0.f, limit = mine ? -1.f : kLargeSum;  // what the scaled scores get; the sum from which on the reference moves
+  const float unscale = 1.f / scale2, slack = kSlack * unscale;
+  float shift = 0.f, far = mine ? -INFINITY : INFINITY;  // what the scaled scores get; the score from which on the reference moves
 
   // ---- what this lane brings of its wavefront's block of a chunk: pieces y = lane, lane + 64, ... < D (some twice where D is no
   // multiple of 64) of the keys (slab, key, half of the slab) and of the values (an element's codes of the 16 keys)
@@ -564,12 +570,32 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
     const u32x4 w = next_values.piece[i];
     ready[2 * i + h] = bf16_of_codes(w[2 * h], w[2 * h + 1], 1.f);
   };
-  float ready_unit;
+  uint32_t ready_exp;  // of key lane % 16 of the block
+  auto unit_of = [&](uint32_t exp) __attribute__((always_inline)) {
+    const int e = static_cast<int>(exp) - 127;
+    return e < -kMostUnit ? -kMostUnit : e > kMostUnit ? kMostUnit : e;
+  };
+  auto put_begin = [&](int slot) __attribute__((always_inline)) {
+    begin[team][slot][member * 16 + lane % 16] = static_cast<float>(unit_of(ready_exp)) * unscale;
+  };
   auto put_values = [&](int chunk, int slot) __attribute__((always_inline)) {
-    const int first = key_begin + 64 * chunk + member * 16;
+    const int first = key_begin + 64 * chunk + member * 16, c = unit_of(ready_exp);
+    uint32_t back = static_cast<uint32_t>(127 - c) << 7;
+    if (__builtin_amdgcn_ballot_w64(c + 127 != static_cast<int>(ready_exp)) != 0) {  // (kept a branch: some value's power of two is out of bounds)
+      asm volatile("");
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int left = __builtin_amdgcn_readlane(static_cast<int>(ready_exp) - 127 - c, 8 * h + e);
+          const float by = __uint_as_float(static_cast<uint32_t>(127 + left) << 23);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) ready[2 * i + h][e] = static_cast<__bf16>(static_cast<float>(ready[2 * i + h][e]) * by);
+        }
+    }
     if (first < lo_min || first + 15 > pos_max) {  // (kept a branch)
       asm volatile("");
-      // slots that no query reads may hold anything, NaN and an infinite unit among them, and their weights of 0 times that have to be 0
+      // slots that no query reads may hold anything, NaN among them, and their weights of 0 times that have to be 0
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         u32x4 keep;
@@ -582,13 +608,12 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
         for (int i = 0; i < kPer; ++i)
           ready[2 * i + h] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, ready[2 * i + h]) & keep);
       }
-      if (first + lane % 16 < lo_min || first + lane % 16 > pos_max) ready_unit = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) *reinterpret_cast<bf16x8*>(values + slot * kSide + (v_at[i] ^ (h * 16))) = ready[2 * i + h];
-    units[team][slot][member * 16 + lane % 16] = ready_unit;
+    undo[team][slot][member * 16 + lane % 16] = static_cast<uint16_t>(back);
   };
 
   // ---- where this lane's operands lie
@@ -600,28 +625,50 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
   const int first_plain = lo_max > key_begin ? (lo_max - key_begin + 63) / 64 : 0;
   f32x16 s[2];
   bf16x8 p[4];
+  auto undo_operand = [&](int slot, int u) __attribute__((always_inline)) {
+    return *reinterpret_cast<const bf16x8*>(&undo[team][slot][u * 16 + half * 8]);
+  };
+  // the scores' first values: register e of tile t is key 32 t + 16 (e / 8) + 8 half + e % 8
+  auto begin_scores = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(&begin[team][slot][32 * t + e / 8 * 16 + 8 * half + e % 8]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[t][e + r] = x[r];
+      }
+  };
   auto add_values = [&](int slot) __attribute__((always_inline)) {
+    f32x16 sums;  // (every register is the row's sum)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sums[r] = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sums = __builtin_amdgcn_mfma_f32_32x32x16_bf16(undo_operand(slot, u), p[u], sums, 0, 0, 0);
 #pragma unroll
     for (int q = 0; q < 4 * DB; ++q) {
       const bf16x8 vf = *reinterpret_cast<const bf16x8*>(values + slot * kSide + vat + q * 1024);
       o[q % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, p[q / DB], o[q % DB], 0, 0, 0);
     }
+    l += sums[0];
   };
-  // ---- the multiplications of a turn: the weights of the turn before with their values (not in the first turn), then the scores
-  // of the keys in `slot`.  Operands are read kAhead multiplications before their own; between them what there is to do for
+  // ---- the multiplications of a turn: the weights of the turn before with 2^-c and their values (not in the first turn), then the
+  // scores of the keys in `slot`.  Operands are read kAhead multiplications before their own; between them what there is to do for
   // the next chunks, piece by piece.  Nothing moves across sched_barrier.
   constexpr int kAhead = 4;
   auto multiply = [&](int slot, int page_ahead, int chunk_ahead, auto with_values) __attribute__((always_inline)) {
-    constexpr int kValues = decltype(with_values)::value ? 4 * DB : 0, kSteps = kValues + 2 * KS;
+    constexpr int kSums = decltype(with_values)::value ? 4 : 0, kScores = kSums + kSums * DB, kSteps = kScores + 2 * KS;
     constexpr int kItems = 4 * kPer + 4;
     const char* from_keys = keys + slot * kSide + kat;
     const char* from_values = values + (1 - slot) * kSide + vat;
     bf16x8 operand[kSteps];
     auto ask = [&](int q) __attribute__((always_inline)) {
-      if (q < kValues) {
-        operand[q] = *reinterpret_cast<const bf16x8*>(from_values + q * 1024);
+      if (q < kSums) {
+        operand[q] = undo_operand(1 - slot, q);
+      } else if (q < kScores) {
+        operand[q] = *reinterpret_cast<const bf16x8*>(from_values + (q - kSums) * 1024);
       } else {  // the two tiles by turns
-        const int t = (q - kValues) % 2, st = (q - kValues) / 2;
+        const int t = (q - kScores) % 2, st = (q - kScores) / 2;
         operand[q] = *reinterpret_cast<const bf16x8*>(from_keys + 2 * t * DB * 1024 + st / 2 * 1024 + ((st % 2 * 2 + half) ^ turn) * 16);
       }
     };
@@ -630,7 +677,7 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
     auto item = [&](int k) __attribute__((always_inline)) {
       if (k < 2 * kPer) ready_values(k / 2, k % 2);
       else if (k < 4 * kPer) put_keys(1 - slot, k / 2 - kPer, k % 2);
-      else if (k == 4 * kPer) ready_unit = __uint_as_float(next_values.exp << 23), at = place_of(page_ahead, chunk_ahead);
+      else if (k == 4 * kPer) ready_exp = next_values.exp, put_begin(1 - slot), at = place_of(page_ahead, chunk_ahead);
       else if (k == 4 * kPer + 1) found = find(chunk_ahead + TEAMS);
       else if (k == 4 * kPer + 2) fetch_keys(at);
       else fetch_values(at);
@@ -638,11 +685,10 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
     if constexpr (TEAMS == 1) {
       // (heads of more than 128 elements: so many steps that the compiler would rather keep their operands in memory than unroll
       // them all with their items between them)
-      if (kValues) add_values(1 - slot);
+      if (kSums) add_values(1 - slot);
+      begin_scores(slot);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
 #pragma unroll
         for (int st = 0; st < KS; ++st)
           s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
@@ -652,22 +698,26 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
       for (int k = 0; k < kItems; ++k) item(k);
       return found;
     }
+    f32x16 sums;  // (every register is the row's sum)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sums[r] = 0.f;
+    if (kSums == 0) begin_scores(slot);
 #pragma unroll
     for (int q = 0; q < kAhead && q < kSteps; ++q) ask(q);
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
     __builtin_amdgcn_sched_barrier(0);
     // before the other team's wavefront, whose vector instructions would keep this one's multiplications waiting
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int q = 0; q < kSteps; ++q) {
       if (q + kAhead < kSteps) ask(q + kAhead);
-      if (q < kValues) {
-        o[q % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand[q], p[q / DB], o[q % DB], 0, 0, 0);
+      if (q < kSums) {
+        sums = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand[q], p[q], sums, 0, 0, 0);
+      } else if (q < kScores) {
+        const int k = q - kSums;
+        o[k % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand[q], p[k / DB], o[k % DB], 0, 0, 0);
+        if (k == 2 * DB) l += sums[0], begin_scores(slot);  // (the sums have left the matrix unit by now)
       } else {
-        const int t = (q - kValues) % 2, st = (q - kValues) / 2;
+        const int t = (q - kScores) % 2, st = (q - kScores) / 2;
         s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand[q], qf[st], s[t], 0, 0, 0);
       }
 #pragma unroll
@@ -678,7 +728,7 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
     __builtin_amdgcn_s_setprio(0);
     return found;
   };
-  auto weigh = [&](int chunk, int slot) __attribute__((always_inline)) {
+  auto weigh = [&](int chunk) __attribute__((always_inline)) {
     const int kb = key_begin + 64 * chunk;
     if (chunk > last_plain || chunk < first_plain) {  // some query does not read all of it
       asm volatile("");  // (stays a branch)
@@ -691,30 +741,13 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
           if (at > q_pos || at < q_lo) s[t][e] = -INFINITY;
         }
     }
-    float sum;
-    auto weights = [&]() __attribute__((always_inline)) {
-      float part[2] = {0.f, 0.f};
-      const float* unit = &units[team][slot][8 * half];
+    float mx = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {  // eight keys of a block
-        const f32x4 by[2] = {*reinterpret_cast<const f32x4*>(unit + 16 * u), *reinterpret_cast<const f32x4*>(unit + 16 * u + 4)};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float w = __builtin_amdgcn_exp2f(fmaf(s[u / 2][u % 2 * 8 + e], scale2, shift));
-          part[e % 2] += w;
-          p[u][e] = static_cast<__bf16>(w * by[e / 4][e % 4]);
-        }
-      }
-      sum = part[0] + part[1];
-    };
-    weights();
-    // The reference is some earlier chunk's maximum.  It only has to keep weights in float32's range: a weight of 2^10 is as exact as
-    // one of 1.  So the maximum is not looked for as long as a row's weights stay small, and o is not rescaled.
-    if (__builtin_amdgcn_ballot_w64(sum > limit) != 0) {
+    for (int e = 1; e < 16; ++e) mx = fmaxf(fmaxf(mx, s[0][e]), s[1][e]);
+    // The reference is some earlier chunk's maximum.  It only has to keep weights in float32's range: one of 2^10 is as exact as one of
+    // 1.  So it moves, and o is rescaled, where a row's scores are far beyond it (or the row has none yet).
+    if (__builtin_amdgcn_ballot_w64(mx > far) != 0) {
       asm volatile("");
-      float mx = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(fmaxf(mx, s[0][e]), s[1][e]);
       const unsigned b = __builtin_bit_cast(unsigned, mx);
       const auto halves = __builtin_amdgcn_permlane32_swap(b, b, false, false);
       const float m_new = fmaxf(m, fmaxf(bits_as_float(halves[0]), bits_as_float(halves[1])));
@@ -722,13 +755,15 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
       const float alpha = __builtin_amdgcn_exp2f((m - m_safe) * scale2);
       m = m_new;
       shift = -m_safe * scale2;
-      limit = m == -INFINITY ? -1.f : kLargeSum;  // (a row without a reference: any sum is over it)
+      far = mine ? m_new + slack : INFINITY;
       l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
-      weights();
     }
-    l += sum;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[u][e] = static_cast<__bf16>(__builtin_amdgcn_exp2f(fmaf(s[u / 2][u % 2 * 8 + e], scale2, shift)));
   };
 
   if (c_first < c_end) {  // the same for every wavefront of the workgroup
@@ -742,7 +777,8 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
     page = find(chunk_of(1));
 #pragma unroll
     for (int i = 0; i < 2 * kPer; ++i) put_keys(0, i / 2, i % 2), ready_values(i / 2, i % 2);
-    ready_unit = __uint_as_float(next_values.exp << 23);
+    ready_exp = next_values.exp;
+    put_begin(0);
     put_values(chunk_of(0), 0);
     at = place_of(page, chunk_of(1));
     fetch_keys(at);
@@ -754,7 +790,7 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
     auto rest = [&](int i) __attribute__((always_inline)) {
       __syncthreads();  // the team has read the values of the turn before
       put_values(chunk_of(i + 1), (i + 1) % 2);
-      if (chunk_of(i) < c_end) weigh(chunk_of(i), i % 2);
+      if (chunk_of(i) < c_end) weigh(chunk_of(i));
       __syncthreads();
     };
     page = multiply(0, page, chunk_of(2), EdgeTag<false>{});
@@ -768,12 +804,7 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
     __syncthreads();  // LDS is read no more
   }
 
-  float total;
-  {
-    const unsigned b = __builtin_bit_cast(unsigned, l);
-    const auto halves = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    total = bits_as_float(halves[0]) + bits_as_float(halves[1]);
-  }
+  float total = l;
   // ---- the teams' results become one: each hands over half of its sums and finishes the other half
   constexpr int kParts = DB * 4, kMine = TEAMS == 2 ? kParts / 2 : kParts;  // of four elements of a lane's row
   const int first_part = TEAMS == 2 ? team * kMine : 0;

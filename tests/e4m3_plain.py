@@ -138,8 +138,11 @@ def attention(step, q, keys, values, heads, scale, window=None, chunk=None):
 
 def allowed(out, size, reach, dim, keys, bf16):
     """How far a kernel's results may be from attention()'s.  float32: sums of dim products and of `keys` weights, each step off by at
-    most 2^-24 of the sum of the terms' sizes; a score's error moves its weight by as much, and the weights' sum too; the
-    exponential is good to 2^-21.  bfloat16 besides: weights are rounded to bfloat16 (2^-8 of each), the result too."""
-    scores = (dim + 4) * 2.0 ** -24 * reach
+    most 2^-24 of the sum of the terms' sizes (a score may begin with up to 40 / log2(e), which is added in the same sum: 64 * 2^-24 more at
+    most); a score's error moves its weight by as much, and the weights' sum too; the exponential is good to 2^-21.
+    bfloat16 besides: the result is rounded (2^-8 of it), and every weight p to p (1 + d), |d| <= 2^-8.  Where the denominator adds up the
+    weights before they are rounded, that is at most 2^-8 size; where it adds up the rounded ones, sum p (1 + d) v / sum p (1 + d) - out =
+    sum p d (v - out) / sum p (1 + d), at most 2^-8 (size + |out|) (1 + 2^-7)."""
+    scores = (dim + 4) * 2.0 ** -24 * reach + 64 * 2.0 ** -24
     fp32 = (2 * scores + 2 * keys * 2.0 ** -24 + 2 * 2.0 ** -21) * size + 2.0 ** -24 * out.abs()
-    return fp32 + (2.0 ** -8 * (size + out.abs()) * (1 + 2.0 ** -7) if bf16 else 0.0)
+    return fp32 + (2.0 ** -8 * (size + 2 * out.abs()) * (1 + 2.0 ** -7) if bf16 else 0.0)

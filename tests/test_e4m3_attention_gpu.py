@@ -151,6 +151,51 @@ def test_one_large_weight_before_many_small_ones(ops):
         assert ((out.cpu().double().view_as(want) - want).abs() <= limit).all()
 
 
+@pytest.mark.parametrize("form", [(14, 2, 64, 16), (28, 4, 128, 16), (8, 1, 256, 32)])
+@pytest.mark.parametrize("sizes", [[-30, 0, 20], [-60, 60], [-100, -99], [70, 72], [0, -117], [None, 0], [None]])
+def test_values_of_very_different_sizes(ops, form, sizes):
+    """Rows of values times 2^size, None: zeros.  (Beyond 40 either way the portions' kernel multiplies the codes themselves.)"""
+    heads, kv, dim, ps = form
+    step = plain.Step([200, 90], [1, 70], ps, seed=8)
+    k_pool, v_pool, scales, keys, values = plain.random_pools(step.pages, kv, dim, ps, step.gen)
+    pick = torch.randint(0, len(sizes), (step.pages, kv, ps), generator=step.gen)
+    by = torch.tensor([0.0 if x is None else 2.0 ** x for x in sizes], dtype=torch.float64)[pick]
+    values, e = plain.quantised(values * by[..., None])
+    codes = (values / 2.0 ** e.double()[..., None]).float().to(plain.E4M3).view(torch.uint8)
+    scales = scales.clone()
+    scales[:, :, 1] = (e + 127).to(torch.uint8)
+    pools = poisoned(step, k_pool, codes.transpose(2, 3).contiguous().view(plain.E4M3), scales)
+    q = (2 * torch.randn(step.n, heads * dim, generator=step.gen)).bfloat16()
+    out = torch.full((step.n, heads * dim), 9.0, dtype=torch.bfloat16, device="cuda")
+    for nsplit in (1, 3):
+        partial = torch.empty(step.n * heads * nsplit * (dim + 2), device="cuda")
+        ops.attention_decode_e4m3(q.cuda(), out, 1, heads, kv, dim, step.positions.cuda(), step.tables.cuda(), *pools, ps, None, dim ** -0.5,
+                                  partial, nsplit)
+        ops.attention_prefill_e4m3(q.cuda(), out, 1, 1, heads, kv, dim, step.cu_q.cuda(), step.ctx_lens.cuda(), step.tables.cuda(), *pools, ps,
+                                   None, dim ** -0.5, partial, nsplit)
+        want, size, reach = plain.attention(step, q, keys, values, heads, dim ** -0.5)
+        # (2^-126: below that bfloat16 numbers and their products have fewer bits)
+        limit = plain.allowed(want, size, reach, dim, 201, True) + 2.0 ** -126
+        assert ((out.cpu().double().view_as(want) - want).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("gain", [30.0, 300.0])
+def test_scores_of_hundreds(ops, gain):
+    """Weights that overflow a type relative to an earlier reference, rising and falling along the keys."""
+    form = heads, kv, dim, ps = 8, 2, 64, 16
+    step = plain.Step([700, 400], [1, 60], ps, seed=9)
+    pools, keys, values, _ = setup(step, form)
+    q = (gain * torch.randn(step.n, heads * dim, generator=step.gen)).bfloat16()
+    out = torch.empty(step.n, heads * dim, dtype=torch.bfloat16, device="cuda")
+    for nsplit in (1, 3):
+        partial = torch.empty(step.n * heads * nsplit * (dim + 2), device="cuda")
+        ops.attention_decode_e4m3(q.cuda(), out, 1, heads, kv, dim, step.positions.cuda(), step.tables.cuda(), *pools, ps, None, 0.125, partial,
+                                  nsplit)
+        ops.attention_prefill_e4m3(q.cuda(), out, 1, 1, heads, kv, dim, step.cu_q.cuda(), step.ctx_lens.cuda(), step.tables.cuda(), *pools, ps,
+                                   None, 0.125, partial, nsplit)
+        check(step, form, out, q, keys, values, None, None)
+
+
 def test_tokens_and_pages_that_are_not_there(ops):
     form = heads, kv, dim, ps = 14, 2, 64, 16
     step = plain.Step([40, 100, 33], [1, 1, 50], ps, seed=4)
