@@ -340,12 +340,16 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
 }
 
 // out[row] = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z, shares in order: a wavefront per row (a token's head), lane z with share
-// z's weight.
+// z's weight.  With `cu_q` a row counts only if its token is one of the sequences': there are no shares of the others.
 template <int D>
-__global__ void __launch_bounds__(kWave) merge_e4m3_kernel(const float* __restrict__ partial, bf16* __restrict__ out, int nsplit) {
+__global__ void __launch_bounds__(kWave)
+    merge_e4m3_kernel(const float* __restrict__ partial, bf16* __restrict__ out, int nsplit, const int32_t* __restrict__ cu_q,
+                      int first_seq, int num_seqs, int heads) {
   constexpr int kBatch = 8, NE = (D + kWave - 1) / kWave;
   const size_t row = blockIdx.x;
   const int lane = threadIdx.x;
+  const int token = first_seq + static_cast<int>(blockIdx.x / heads);
+  const int from = cu_q ? cu_q[first_seq] : 0, to = cu_q ? cu_q[first_seq + num_seqs] : token + 1;
   const float* src = partial + row * nsplit * D;
   float2 mine = make_float2(-INFINITY, 0.f);
   if (lane < nsplit) mine = *reinterpret_cast<const float2*>(partial + static_cast<size_t>(gridDim.x) * nsplit * D + (row * nsplit + lane) * 2);
@@ -372,6 +376,7 @@ __global__ void __launch_bounds__(kWave) merge_e4m3_kernel(const float* __restri
     }
     if (z0 + kBatch < nsplit) fetch(z0 + kBatch);
   }
+  if (token < from || token >= to) return;
   const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
   for (int e = 0; e < NE; ++e)
@@ -915,8 +920,9 @@ int check_mfma(const char* who, int heads, int kv_heads, int head_dim, int page_
 uint32_t page_magic(int page_size) { return static_cast<uint32_t>(((1ull << 32) + page_size - 1) / page_size); }
 
 template <int D>
-void merge_e4m3(int rows, hipStream_t s, const float* partial, void* out, int nsplit) {
-  merge_e4m3_kernel<D><<<rows, kWave, 0, s>>>(partial, static_cast<bf16*>(out), nsplit);
+void merge_e4m3(int rows, hipStream_t s, const float* partial, void* out, int nsplit, const int32_t* cu_q = nullptr, int first_seq = 0,
+                int num_seqs = 0, int heads = 1) {
+  merge_e4m3_kernel<D><<<rows, kWave, 0, s>>>(partial, static_cast<bf16*>(out), nsplit, cu_q, first_seq, num_seqs, heads);
 }
 
 #define E4M3_BY_DIM(head_dim, CASE) \
@@ -997,7 +1003,9 @@ extern "C" int shk_attention_prefill_e4m3(const void* q, int q_stride, void* out
   constexpr int kTeams##D = D <= 128 ? 2 : 1;                                                                           \
   (page_size == 16 ? attention_portion_e4m3_kernel<D, kTeams##D, 16> : attention_portion_e4m3_kernel<D, kTeams##D, 0>)   \
       <<<static_cast<unsigned>(count), kTeams##D * 4 * kWave, 0, s>>>(a);                                               \
-  if (nsplit > 1) merge_e4m3<D>(tokens * heads, s, partial, static_cast<bf16*>(out) + static_cast<size_t>(first_seq) * heads * D, nsplit)
+  if (nsplit > 1)                                                                                                        \
+  merge_e4m3<D>(tokens * heads, s, partial, static_cast<bf16*>(out) + static_cast<size_t>(first_seq) * heads * D, nsplit, cu_q, \
+                first_seq, num_seqs, heads)
   E4M3_BY_DIM(head_dim, LAUNCH)
 #undef LAUNCH
   SHK_LAUNCH_CHECK("attention_prefill_e4m3");

@@ -312,3 +312,21 @@ def test_refusals_of_the_matrix_kernels(ops):
     assert not ops.attention_e4m3_supports_mfma(14, 2, 64, 8, 14 * 64)
     assert not ops.attention_e4m3_supports_mfma(129, 1, 64, 16, 129 * 64)
     assert not ops.attention_e4m3_supports_mfma(14, 2, 64, 16, 14 * 64 + 4)
+
+
+@pytest.mark.parametrize("form", [(14, 2, 64, 16), (28, 4, 128, 16), (8, 1, 256, 32)])
+@pytest.mark.parametrize("nsplit", [1, 2, 5])
+def test_rows_that_belong_to_no_sequence_stay(ops, form, nsplit):
+    """A batch padded at its end, and one whose last sequences are not asked for."""
+    heads, kv, dim, ps = form
+    step = plain.Step([0, 70, 200, 5], [1, 40, 33, 20], ps, seed=8)
+    pools, keys, values, q = setup(step, form)
+    padded = torch.cat([q, torch.randn(37, heads * dim, generator=step.gen).bfloat16()]).cuda()
+    partial = torch.empty(padded.shape[0] * heads * nsplit * (dim + 2), device="cuda")
+    for count, rows in ((3, step.n), (2, step.n - 20), (1, 41)):
+        out = torch.full((step.n + 37, heads * dim), 9.0, dtype=torch.bfloat16, device="cuda")
+        partial.fill_(float("nan"))
+        ops.attention_prefill_e4m3(padded, out, 1, count, heads, kv, dim, step.cu_q.cuda(), step.ctx_lens.cuda(), step.tables.cuda(), *pools,
+                                   ps, None, dim ** -0.5, partial, nsplit)
+        assert (out[:1] == 9).all() and (out[rows:] == 9).all()
+        check(step, form, out[:step.n], q, keys, values, None, None, slice(1, rows))
