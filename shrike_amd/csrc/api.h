@@ -254,9 +254,10 @@ int shk_qkv_store(void* qkv, int dtype, int n, int heads, int kv_heads, int head
 // A quantised cache (e4m3.h): keys and values as E4M3 codes, `scales` [num_pages, kv_heads, 2, page_size] bytes, the biased
 // exponents of a power of two per token and head, the keys' before the values'; pools of bytes in the layouts of shk_rope_kv_store.
 // In every call: tables is [num_seqs, table_stride]; a position below 0, or one whose page is beyond the tables or outside the
-// pool, is a token that is not there.
+// pool, is a token that is not there.  Pools are 16-byte aligned.
 // shk_rope_kv_store_e4m3: shk_rope_kv_store into such a cache, angles formed in float64; keys and values are quantised from float32.
 // Queries go to q_out, rows q_ld elements apart (qkv itself, q_ld its width: in place).  Tokens that are not there leave the pools alone.
+// A call holds a position of a sequence once, and no page that another call running at the same time writes.
 // shk_kv_read_e4m3: rows [n, kv_heads * head_dim] of `dtype` of the tokens (token_seq[t], positions[t]); NaN for one that is not there.
 // shk_attention_e4m3: shk_attention over such a cache (window, chunk; no cap, sinks or bias); scale > 0.  Keys that are not there
 // are not read; a query without any key gets zeros.
@@ -274,7 +275,8 @@ int shk_attention_e4m3(const void* q, int q_stride, void* out, int dtype, int n,
                        int chunk, float scale, void* stream);
 
 // The same on the matrix units for bfloat16, where shk_attention_e4m3_supports_mfma says so (head_dim a multiple of 32 up to 256,
-// page_size of 16, up to 128 query heads a key/value head, q rows 16-byte aligned).
+// page_size of 16, up to 128 query heads a key/value head, q rows 16-byte aligned; out and partial are too).  Here every key that a
+// query reads has to be there: a page outside the pool or the tables is not followed, but another one is read in its place.
 // shk_attention_decode_e4m3: sequence s has one query token, row s of q, at positions[s]; nsplit > 1 workgroups share its keys.
 // shk_attention_prefill_e4m3: rows first_seq .. n - 1 of q and out are the new tokens of sequences first_seq .. first_seq +
 // num_seqs - 1 (those before have a token each): rows cu_q[s] .. cu_q[s + 1], at the end of ctx_lens[s] tokens.  Other rows stay.

@@ -575,6 +575,8 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
     const u32x4 w = next_values.piece[i];
     ready[2 * i + h] = bf16_of_codes(w[2 * h], w[2 * h + 1], 1.f);
   };
+  const int last_plain = (pos_min + 1 - key_begin) / 64 - 1;  // the last chunk that every query reads whole, and the first
+  const int first_plain = lo_max > key_begin ? (lo_max - key_begin + 63) / 64 : 0;
   uint32_t ready_exp;  // of key lane % 16 of the block
   auto unit_of = [&](uint32_t exp) __attribute__((always_inline)) {
     const int e = static_cast<int>(exp) - 127;
@@ -586,18 +588,6 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
   auto put_values = [&](int chunk, int slot) __attribute__((always_inline)) {
     const int first = key_begin + 64 * chunk + member * 16, c = unit_of(ready_exp);
     uint32_t back = static_cast<uint32_t>(127 - c) << 7;
-    if (__builtin_amdgcn_ballot_w64(c + 127 != static_cast<int>(ready_exp)) != 0) {  // (kept a branch: some value's power of two is out of bounds)
-      asm volatile("");
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int left = __builtin_amdgcn_readlane(static_cast<int>(ready_exp) - 127 - c, 8 * h + e);
-          const float by = __uint_as_float(static_cast<uint32_t>(127 + left) << 23);
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) ready[2 * i + h][e] = static_cast<__bf16>(static_cast<float>(ready[2 * i + h][e]) * by);
-        }
-    }
     if (first < lo_min || first + 15 > pos_max) {  // (kept a branch)
       asm volatile("");
       // slots that no query reads may hold anything, NaN among them, and their weights of 0 times that have to be 0
@@ -614,6 +604,39 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
           ready[2 * i + h] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, ready[2 * i + h]) & keep);
       }
     }
+    if (chunk > last_plain || chunk < first_plain) {  // (kept a branch: some query does not read all of it)
+      asm volatile("");
+      // A value's NaN must not reach the queries whose weight for it is 0.  So it counts as 0, and its score begins as NaN: that is
+      // its weight where it is read.  (Codes are at most 448, so bits 13 and 14 of their bfloat16 numbers are both set in NaN alone.)
+      auto nan_bits = [](u32x4 w) { return w & (w << 1) & 0x40004000u; };
+      u32x4 found[2] = {};
+#pragma unroll
+      for (int i = 0; i < 2 * kPer; ++i) found[i % 2] |= nan_bits(__builtin_bit_cast(u32x4, ready[i]));
+      const u32x4 any = found[0] | found[1];
+      if (__builtin_amdgcn_ballot_w64((any[0] | any[1] | any[2] | any[3]) != 0) != 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (__builtin_amdgcn_ballot_w64((found[h][e / 2] >> (e % 2 * 16) & 0x4000u) != 0) == 0) continue;
+            if (lane % 16 == 8 * h + e) begin[team][slot][member * 16 + lane % 16] = __builtin_nanf("");
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) ready[2 * i + h][e] = static_cast<__bf16>(0.f);
+          }
+      }
+    }
+    if (__builtin_amdgcn_ballot_w64(c + 127 != static_cast<int>(ready_exp)) != 0) {  // (kept a branch: some value's power of two is out of bounds)
+      asm volatile("");
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int left = __builtin_amdgcn_readlane(static_cast<int>(ready_exp) - 127 - c, 8 * h + e);
+          const float by = __uint_as_float(static_cast<uint32_t>(127 + left) << 23);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) ready[2 * i + h][e] = static_cast<__bf16>(static_cast<float>(ready[2 * i + h][e]) * by);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
 #pragma unroll
@@ -626,8 +649,6 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
   const int turn = key % 16 / 4;
   const int kat = key / 16 * DB * 1024 + key % 16 * 64, vat = col * 32 + (half ^ (col / 8 % 2)) * 16;
 
-  const int last_plain = (pos_min + 1 - key_begin) / 64 - 1;  // the last chunk that every query reads whole, and the first
-  const int first_plain = lo_max > key_begin ? (lo_max - key_begin + 63) / 64 : 0;
   f32x16 s[2];
   bf16x8 p[4];
   auto undo_operand = [&](int slot, int u) __attribute__((always_inline)) {
@@ -917,6 +938,10 @@ int check_mfma(const char* who, int heads, int kv_heads, int head_dim, int page_
   return 0;
 }
 
+bool aligned16(const void* a, const void* b, const void* c) {
+  return (reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) % 16 == 0;
+}
+
 uint32_t page_magic(int page_size) { return static_cast<uint32_t>(((1ull << 32) + page_size - 1) / page_size); }
 
 template <int D>
@@ -956,7 +981,8 @@ extern "C" int shk_attention_decode_e4m3(const void* q, int q_stride, void* out,
   if (num_seqs == 0) return 0;
   SHK_REQUIRE(q && out && positions && tables && k_pool && v_pool && scales && (partial || nsplit == 1),
               "attention_decode_e4m3: null pointer");
-  SHK_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0, "attention_decode_e4m3: rows of q must be 16-byte aligned");
+  SHK_REQUIRE(aligned16(q, out, partial) && aligned16(k_pool, v_pool, scales),
+              "attention_decode_e4m3: rows, pools and the scratch must be 16-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int head_tiles = (heads / kv_heads + 15) / 16;
   const dim3 grid(kv_heads * head_tiles, num_seqs, nsplit);
@@ -985,8 +1011,8 @@ extern "C" int shk_attention_prefill_e4m3(const void* q, int q_stride, void* out
   if (num_seqs == 0 || n == first_seq) return 0;
   SHK_REQUIRE(q && out && cu_q && ctx_lens && tables && k_pool && v_pool && scales && (partial || nsplit == 1),
               "attention_prefill_e4m3: null pointer");
-  SHK_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
-              "attention_prefill_e4m3: rows must be 16-byte aligned");
+  SHK_REQUIRE(aligned16(q, out, partial) && aligned16(k_pool, v_pool, scales),
+              "attention_prefill_e4m3: rows, pools and the scratch must be 16-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int tokens = n - first_seq, group = heads / kv_heads;
   const int queries = kPortionRows / group;

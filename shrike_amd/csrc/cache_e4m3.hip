@@ -474,6 +474,11 @@ using namespace shk;
   SHK_REQUIRE(n >= 0 && kv_heads > 0 && head_dim > 0 && head_dim <= kMaxDim, who ": n=%d, kv_heads=%d, head_dim=%d (1..%d)", n, \
               kv_heads, head_dim, kMaxDim)
 
+// The kernels move up to 16 bytes of a page at a time.
+static bool aligned_pools(const void* k, const void* v, const void* scales) {
+  return (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(scales)) % 16 == 0;
+}
+
 extern "C" int shk_rope_kv_store_e4m3(const void* qkv, int dtype, int n, int heads, int kv_heads, int head_dim, int rot_dim,
                                       const float* inv_freq, const int32_t* positions, const int32_t* token_seq,
                                       const int32_t* tables, int table_stride, int num_seqs, void* k_pool, void* v_pool,
@@ -492,6 +497,8 @@ extern "C" int shk_rope_kv_store_e4m3(const void* qkv, int dtype, int n, int hea
                             num_seqs > 0),
               "rope_kv_store_e4m3: bad cache (page_size=%d, num_pages=%d, table_stride=%d, num_seqs=%d)", page_size, num_pages,
               table_stride, num_seqs);
+  SHK_REQUIRE(!write_kv || aligned_pools(k_pool, v_pool, scales), "rope_kv_store_e4m3: pools must be 16-byte aligned");
+  SHK_REQUIRE(static_cast<long long>(n) * (heads + 2LL * kv_heads) < (1LL << 31), "rope_kv_store_e4m3: too many tokens: %d", n);
   const StoreArgs a{qkv, parts, bias, q_out, inv_freq, positions, token_seq, tables, n, heads, kv_heads, head_dim, rot_dim,
                     splits, pairing, v_from_k, q_ld, table_stride, num_seqs, write_kv, magnitude};
   const E4m3Pools pools{static_cast<uint8_t*>(k_pool), static_cast<uint8_t*>(v_pool), static_cast<uint8_t*>(scales), page_size,
@@ -504,7 +511,6 @@ extern "C" int shk_rope_kv_store_e4m3(const void* qkv, int dtype, int n, int hea
     kernel<<<value_groups + n, kStoreThreads, 0, s>>>(a, pools, value_groups);
   } else {
     const int row_groups = (heads + (write_kv ? 2 * kv_heads : 0) + kStoreWaves - 1) / kStoreWaves;
-    SHK_REQUIRE(static_cast<long long>(n) * row_groups < (1LL << 31), "rope_kv_store_e4m3: too many tokens: %d", n);
     if (dtype == kF32)
       store_e4m3_kernel<float><<<n * row_groups, kStoreThreads, 0, s>>>(a, pools, row_groups);
     else
@@ -523,7 +529,9 @@ extern "C" int shk_kv_read_e4m3(void* k_out, void* v_out, int dtype, int n, int 
               "kv_read_e4m3: bad cache (page_size=%d, num_pages=%d, table_stride=%d, num_seqs=%d)", page_size, num_pages, table_stride,
               num_seqs);
   if (n == 0) return 0;
+  SHK_REQUIRE(static_cast<long long>(n) * kv_heads < (1LL << 31), "kv_read_e4m3: too many tokens: %d", n);
   SHK_REQUIRE(k_out && v_out && positions && token_seq && tables && k_pool && v_pool && scales, "kv_read_e4m3: null pointer");
+  SHK_REQUIRE(aligned_pools(k_pool, v_pool, scales), "kv_read_e4m3: pools must be 16-byte aligned");
   // (read only; the struct serves the writer too)
   const E4m3Pools pools{static_cast<uint8_t*>(const_cast<void*>(k_pool)), static_cast<uint8_t*>(const_cast<void*>(v_pool)),
                         static_cast<uint8_t*>(const_cast<void*>(scales)), page_size, num_pages, kv_heads, head_dim};

@@ -330,3 +330,58 @@ def test_rows_that_belong_to_no_sequence_stay(ops, form, nsplit):
                                    ps, None, dim ** -0.5, partial, nsplit)
         assert (out[:1] == 9).all() and (out[rows:] == 9).all()
         check(step, form, out[:step.n], q, keys, values, None, None, slice(1, rows))
+
+
+@pytest.mark.parametrize("form", [(4, 2, 64, 16), (6, 2, 128, 32), (4, 2, 96, 16), (4, 2, 256, 16)])
+@pytest.mark.parametrize("window, chunk", [(None, None), (30, None), (None, 70)])
+@pytest.mark.parametrize("nsplit", [1, 3])
+def test_a_nan_in_a_value_reaches_the_rows_that_read_it_and_no_others(ops, form, window, chunk, nsplit):
+    """Also where a neighbouring query of the same workgroup reads it."""
+    heads, kv, dim, ps = form
+    step = plain.Step([40, 45, 100], [1, 1, 150], ps, seed=9)
+    pools, keys, values, q = setup(step, form)
+    v = pools[1].view(torch.uint8)
+    at = {0: 40, 1: 20, 2: 137}
+    for seq, key in at.items():
+        v[step.tables[seq, key // ps].long(), seq % 2, :, key % ps] = 0x7f if seq else 0xff
+        values[step.tables[seq, key // ps].long(), seq % 2, key % ps] = 0.0
+    partial = torch.empty(step.n * heads * nsplit * (dim + 2), device="cuda")
+    out = torch.zeros(step.n, heads * dim, dtype=torch.bfloat16, device="cuda")
+    where = (step.tables.cuda(), *pools, ps, window, dim ** -0.5)
+    ops.attention_decode_e4m3(q.cuda(), out, 2, heads, kv, dim, step.positions.cuda(), *where, partial, nsplit, chunk=chunk)
+    ops.attention_prefill_e4m3(q.cuda(), out, 2, 1, heads, kv, dim, step.cu_q.cuda(), step.ctx_lens.cuda(), *where, partial, nsplit, chunk=chunk)
+    want = torch.zeros(step.n, heads, dtype=torch.bool)
+    for t in range(step.n):
+        seq, pos = int(step.token_seq[t]), int(step.positions[t])
+        key = at[seq]
+        if key <= pos and (not window or pos - key < window) and (not chunk or key // chunk == pos // chunk):
+            want[t, seq % 2 * heads // 2:(seq % 2 + 1) * heads // 2] = True
+    bad = out.cpu().view(step.n, heads, dim).isnan()
+    assert torch.equal(bad.any(-1), want) and torch.equal(bad.all(-1), want)
+    clean = torch.where(bad, 0.0, out.cpu().float().view(step.n, heads, dim)).bfloat16().view(step.n, -1)
+    want_off, size, reach = plain.attention(step, q, keys, values, heads, dim ** -0.5, window, chunk)
+    off = (clean.double().view_as(want_off) - want_off).abs()
+    limit = plain.allowed(want_off, size, reach, dim, 250, True)
+    assert (off <= limit)[~want].all()
+    general = torch.empty_like(out)
+    ops.attention_e4m3(q.cuda(), general, heads, kv, dim, step.positions.cuda(), step.token_seq.cuda(), *where, chunk=chunk)
+    assert torch.equal(general.cpu().view(step.n, heads, dim).isnan().any(-1), want)
+
+
+def test_refusals_of_what_is_not_aligned(ops):
+    from shrike_amd.kernels.lib import KernelError
+
+    form = heads, kv, dim, ps = 14, 2, 64, 16
+    step = plain.Step([40, 20], [1, 9], ps, seed=10)
+    pools, _, _, q = setup(step, form)
+    q = q.cuda()
+    scratch = torch.empty(step.n * heads * 2 * (dim + 2) + 1, device="cuda")
+    shifted = torch.empty(step.n * heads * dim + 1, dtype=torch.bfloat16, device="cuda")[1:].view(step.n, -1)
+    out = torch.empty(step.n, heads * dim, dtype=torch.bfloat16, device="cuda")
+    single = (step.positions.cuda(), step.tables.cuda(), *pools, ps, None, 0.1)
+    runs = (step.cu_q.cuda(), step.ctx_lens.cuda(), step.tables.cuda(), *pools, ps, None, 0.1)
+    for args in ((shifted, scratch[:-1]), (out, scratch[1:])):
+        with pytest.raises(KernelError, match="aligned"):
+            ops.attention_decode_e4m3(q, args[0], 1, heads, kv, dim, *single, args[1], 2)
+        with pytest.raises(KernelError, match="aligned"):
+            ops.attention_prefill_e4m3(q, args[0], 1, 1, heads, kv, dim, *runs, args[1], 2)
