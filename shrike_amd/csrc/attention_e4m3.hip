@@ -92,7 +92,14 @@ __global__ void __launch_bounds__(kGeneralThreads)
 // 16 bytes of a page for every element, one load, and are its operand of the second product as they come.  Of its keys' rows a
 // lane loads 16 bytes too, of two slabs of 32 elements at a time (the order of the elements within a product is free as long
 // as both operands agree); a head size with an odd number of slabs takes its last one in pieces of 8.
-// Keys become bfloat16 with their power of two, values without: theirs joins the weight, before that is rounded to bfloat16.
+// Keys become bfloat16 with their power of two, values without: theirs joins the weight, before that is rounded to bfloat16 (an operand
+// of the matrix unit; maximum, sums and products stay float32).
+//
+// Many keys are bound by memory: 8 sequences of 16,000 keys, 40 heads of 128 over 8 (264 MB) 52 us, what a copy of as many bytes takes.
+// A wavefront has one chunk in flight and takes 1.4 us a chunk then; one sequence of 333 keys is one chunk a wavefront, 6.2 us, most of it
+// the way position -> page -> codes.  64 sequences of 61 to 4,000 keys 34 us where their bytes alone would take 26: they end at
+// different times.  Eight wavefronts a workgroup instead of four: 8 sequences of 2,060 keys of 4 heads 14.8 us unshared (16.3), and in the
+// shares that serve them best 11.6 (11.2); 128 of 100 to 900 22 (17).
 template <int D>
 struct KeyBlock {
   static constexpr int kPairs = D / 64, kOdd = D / 32 % 2;
@@ -406,6 +413,14 @@ __global__ void __launch_bounds__(kWave)
 //
 // The workgroups find their queries themselves, a sequence's last queries (which read the most keys) first, so a step needs no
 // lists from the host.
+//
+// 28 heads of 128 over 4: 512 tokens at 16,000 keys 136 us (880 TFLOP/s), 2,048 at 0 50 (600; with one team, conversions in a phase of
+// their own and a reference that moves with every chunk: 513 and 135).  A turn of both teams, 128 keys, takes 2.1 to 2.4 us.  What bounds it: 44
+// operands of 16 bytes a lane and chunk out of LDS (1,400 cycles for the four wavefronts of a team, where their multiplications take
+// 1,150), instructions of any kind (with two wavefronts on a SIMD unit one every 5 cycles or so), and the clock, 1.9 GHz under this load.  Around
+// the turns 4.5 us until the first multiplication (sequence -> page -> codes -> LDS) and 2 us to join and leave, which is most of a
+// short portion: 4 of 17 tokens at 700 to 1,900 keys 11 us.  Keeping codes in LDS instead would spare 16 of the 44 reads, but every wavefront
+// would convert the whole chunk, 96 instructions more.
 constexpr int kPortionRows = 128;
 constexpr float kSlack = 10.f;  // log2 of the largest weight relative to the reference: beyond it moves
 constexpr int kMostUnit = 40;

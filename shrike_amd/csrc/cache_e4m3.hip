@@ -155,7 +155,8 @@ __device__ __forceinline__ void turn4(uint32_t (&w)[4]) {
 // Many tokens of bfloat16 rows that turn whole, (i, i + head_dim / 2) together, head_dim a multiple of 32.  Queries and keys: a
 // workgroup per token, kLanes lanes a head with eight pairs each (16-byte loads, 8-byte pieces of codes) and a table of cosines.
 // Values: 16 neighbouring tokens of a step and one key/value head a workgroup; their codes turn in LDS, so that what lies side by side in a page
-// leaves in one piece, 16 bytes where the tokens fill a block of 16.  What bounds it is traffic: a token of 28 heads over 4 moves 17 KiB.
+// leaves in one piece, 16 bytes where the tokens fill a block of 16.  What bounds it is traffic: a token of 40 heads over 8 of 128 moves
+// 26 KiB; 8,192 of them 55 us (a copy of as many bytes: 42), 180 in the kernel above.  512 tokens 7.1 us, which is launch and latency.
 constexpr int kBlock = 16;
 
 template <int LANES>
@@ -370,8 +371,8 @@ __global__ void __launch_bounds__(kStoreThreads)
 // The same for heads of a multiple of 32 elements: 16 neighbouring tokens of the call and one head a workgroup.  Keys go from 8-byte
 // pieces of a slab into 16-byte pieces of a row (of bfloat16).  Values of tokens that fill a block of 16 come in whole lines and turn
 // on their way, four by four bytes in registers and the rest through LDS; those of other tokens byte by byte, all at once: what a few
-// scattered tokens cost is one load's way.  128,000 tokens of 4 heads of 128 131 us with the values' bytes put into LDS one by
-// one, a thread an element.
+// scattered tokens cost is one load's way (333 tokens of 2 heads of 64 3.9 us).  128,000 tokens of 4 heads of 128, 394 MB, 85 us (a copy of as
+// many bytes: 77); with the values' bytes put into LDS one by one, a thread an element, 131.
 constexpr int kReadThreads = 128;
 
 template <typename T>
