@@ -949,7 +949,8 @@ int check_mfma(const char* who, int heads, int kv_heads, int head_dim, int page_
               q_stride);
   SHK_REQUIRE(num_pages > 0 && table_stride > 0, "%s: bad cache sizes num_pages=%d table_stride=%d", who, num_pages, table_stride);
   SHK_REQUIRE(nsplit >= 1 && nsplit <= kMaxShares, "%s: %d shares of the keys, 1..%d are built", who, nsplit, kMaxShares);
-  SHK_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive, got %g", who, scale);
+  // (sums of exponents with 1 / scale have to stay in float32's range)
+  SHK_REQUIRE(scale >= 0x1p-100f && scale <= 0x1p100f, "%s: scale must be positive, 2^-100 to 2^100, got %g", who, scale);
   return 0;
 }
 

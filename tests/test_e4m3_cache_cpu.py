@@ -132,3 +132,22 @@ def test_launch_plans(heads, kv):
         longest = max(a + n for a, n in zip(starts, lens))
         assert 1 <= e4m3_portion_splits(lens, starts, heads, kv, 128, 1 << 40) <= min(64, -(-longest // 256))
         assert e4m3_portion_splits(lens, starts, heads, kv, 128, 100) == 1  # a window of 100 keys is not shared
+
+
+def test_refusals_of_the_matrix_kernels_before_any_launch(lib):
+    P = None
+
+    def decode(seqs=2, heads=4, kv=2, dim=64, q_ld=256, ps=16, pages=9, stride=3, rows=2, scale=0.1, nsplit=1):
+        return (P, q_ld, P, seqs, heads, kv, dim, P, P, stride, rows, P, P, P, ps, pages, 0, 0, scale, P, nsplit, P)
+
+    def portions(n=9, first=1, seqs=1, heads=4, kv=2, dim=64, q_ld=256, ps=16, pages=9, stride=3, rows=2, scale=0.1, nsplit=1):
+        return (P, q_ld, P, n, first, seqs, heads, kv, dim, P, P, P, stride, rows, P, P, P, ps, pages, 0, 0, scale, P, nsplit, P)
+
+    for name, args in (("shk_attention_decode_e4m3", decode), ("shk_attention_prefill_e4m3", portions)):
+        assert getattr(lib, name)(*args(seqs=0)) == 0
+        for bad, part in ((args(dim=80), "not built"), (args(ps=24), "not built"), (args(kv=3), "not built"), (args(q_ld=260), "not built"),
+                          (args(pages=0), "num_pages=0"), (args(stride=0), "table_stride=0"), (args(nsplit=0), "shares"),
+                          (args(nsplit=65), "shares"), (args(rows=0), "tables of 0"), (args(scale=0.0), "positive"),
+                          (args(scale=1e-38), "positive"), (args(scale=1e38), "positive"), (args(scale=float("nan")), "positive"),
+                          (args(), "null pointer")):
+            refused(lib, name, bad, part)
