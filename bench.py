@@ -316,7 +316,7 @@ def measure_peaks(device="cuda:0") -> dict:
 
 # the functions of shrike_amd.kernels.ops that launch a step's kernels
 TIMED_OPS = ("embed", "add_rmsnorm", "act_mul", "gemm", "gemm_f32_tiled_weight", "gemm_f32_groups", "gemm_f32_gated", "latent_prompt",
-             "gemm_tiled_weight", "few_stream", "few_gated", "few_heads", "rope_kv_store", "attention",
+             "gemm_tiled_weight", "few_stream", "few_gated", "few_heads", "few_plain", "rope_kv_store", "attention",
              "attention_decode", "attention_prefill", "attention_prefill_shared", "argmax", "sample",
              "add_deltas", "add_normed_rmsnorm", "act_mul_rows", "add_rows", "embed_pairs", "qkv_store",
              "latent_prepare", "rotate_heads", "latent_attention", "latent_attention_mfma", "gemm_batched", "mlstm_scan", "headnorm_gate",
@@ -332,8 +332,8 @@ def timed_label(name: str, args, kwargs) -> str:
     if name in ("gemm_tiled_weight", "few_stream", "few_gated", "gemm_f32_groups", "gemm_f32_gated"):
         kind = "gemm" if name == "gemm_tiled_weight" else name
         return f"{kind} {args[2]}x{args[3]}" + (" gated" if kwargs.get("gated") else "")
-    if name == "few_heads":  # (rows, weights, k, out, ..): out is as wide as the matrix has rows
-        return f"few_heads {args[3].shape[1]}x{args[2]}"
+    if name in ("few_heads", "few_plain"):  # (rows, weights, k, out, ..): out is as wide as the matrix has rows
+        return f"{name} {args[3].shape[1]}x{args[2]}"
     return name
 
 

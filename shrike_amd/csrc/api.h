@@ -170,9 +170,11 @@ int shk_gemm_bf16_tiles(int n, int m, int k, int gated, int ksplit, int aligned,
 // shk_few_heads: (a @ w^T) / rms + bias as the [n, (heads + 2 kv_heads) * head_dim] projections of shk_rope_kv_store, which
 // are rotated whole (pairs (i, i + head_dim / 2)): queries go to out's query columns (its others are left alone), keys and
 // values to their pages as there.  sums null: rows that are normed already.  head_dim a multiple of 16.
+// shk_few_plain: out[n, m] = (a @ w^T) / rms + bias in float32, which is one of shk_rope_kv_store_e4m3's parts; m a multiple of 16.
 int shk_few_stream_sums(int n, int m, int k);
 int shk_few_gated_takes(int n, int m, int k);
 int shk_few_heads_takes(int n, int m, int k);
+int shk_few_plain_takes(int n, int m, int k);
 int shk_few_stream(const void* a, int lda, int n, int k, const void* wt, int m, const float* bias, float* resid,
                    const float* weight, void* rows, float* sums, void* stream);
 int shk_few_gated(const void* a, int lda, int n, int k, const void* wt, const float* sums, int count, float eps,
@@ -182,6 +184,8 @@ int shk_few_heads(const void* a, int lda, int n, int k, const void* wt, const fl
                   const int32_t* positions, const int32_t* token_seq, const int32_t* tables, int table_stride,
                   void* k_pool, void* v_pool, int page_size, int num_pages, int write_kv, float magnitude,
                   void* stream);
+int shk_few_plain(const void* a, int lda, int n, int k, const void* wt, const float* sums, int count, float eps,
+                  const float* bias, float* out, int m, void* stream);
 
 // The matrix instruction alone, for measuring its rate on operands of a given kind:
 // workgroups x 4 wavefronts each multiply, iters times, a 64 x 64 x 32 block

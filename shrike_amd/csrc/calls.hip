@@ -72,6 +72,7 @@ const Launcher kLaunchers[] = {
     SHK_LAUNCHER(shk_few_stream),
     SHK_LAUNCHER(shk_few_gated),
     SHK_LAUNCHER(shk_few_heads),
+    SHK_LAUNCHER(shk_few_plain),
     SHK_LAUNCHER(shk_rope_kv_store),
     SHK_LAUNCHER(shk_attention),
     SHK_LAUNCHER(shk_attention_decode_bf16),

@@ -222,13 +222,14 @@ __global__ void __launch_bounds__(kFewWaves* kWave)
 // Projections to queries, keys and values.  A workgroup forms 16 rows of the stacked matrix: of a query or key head 8 elements
 // of the first half and their partners of the second, so that the rotation finds both, of the values 16 elements in a
 // row.  The last wavefront multiplies nothing: it looks up pages and forms cosines and sines meanwhile.
+// `plain`: the rows leave as they are, in float32 (a matrix of no heads, head_dim its height), for a cache write that has to see a whole head.
 template <int C, int LOADS>
 __global__ void __launch_bounds__(kFewWaves* kWave)
     few_heads_kernel(FewRows x, const u32x4* __restrict__ wt, int ktiles, FewScale scaled, const float* __restrict__ bias,
                      bf16* __restrict__ out, int heads, int kv_heads, int head_dim, const float* __restrict__ inv_freq,
                      const int32_t* __restrict__ positions, const int32_t* __restrict__ token_seq,
                      const int32_t* __restrict__ tables, int table_stride, bf16* __restrict__ k_pool, bf16* __restrict__ v_pool,
-                     int page_size, int num_pages, int write_kv, float magnitude) {
+                     int page_size, int num_pages, int write_kv, float magnitude, float* __restrict__ plain) {
   extern __shared__ f32x4 red[];  // [waves][64], then the squares' sums by wavefront [waves + 1][16]
   __shared__ float cosine[16][8], sine[16][8];
   __shared__ int page_of[16], slot_of[16];
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kFewWaves* kWave)
   squares.load(scaled, x.n);
   if (wave == waves) {
     if (LOADS) squares.leave(part);
-    if (lane < 16 && few_first<1>() + lane < x.n) {
+    if (!plain && lane < 16 && few_first<1>() + lane < x.n) {
       const int pos = positions[few_first<1>() + lane];
       int page = -1;
       if (write_kv && head >= heads)
@@ -278,6 +279,12 @@ __global__ void __launch_bounds__(kFewWaves* kWave)
   if (inside >= 16 || token >= x.n) return;
   const float s = squares.scale(scaled, part, inside, waves + 1);
   const float x1 = few_sum(red, kWave, i, inside, waves) * s + b1, x2 = few_sum(red, kWave, i + 8, inside, waves) * s + b2;
+  if (plain) {
+    float* row = plain + static_cast<size_t>(token) * head_dim;
+    row[first + i] = x1;
+    row[second + i] = x2;
+    return;
+  }
   const float c = turned ? cosine[inside][i] : 1.f, t = turned ? sine[inside][i] : 0.f;
   const float o1 = turned ? x1 * c - x2 * t : x1, o2 = turned ? x2 * c + x1 * t : x2;
   if (head < heads) {
@@ -374,6 +381,14 @@ extern "C" int shk_few_heads_takes(int n, int m, int k) {
   return n <= kFewHeadsTokens && (counted_tokens(n) + 15LL) / 16 * m * k <= (n <= kFewTokens ? kFewHeadsReadFew : kFewHeadsRead);
 }
 
+// Rows that a kernel of their own rotates and stores: small matrices alone, where the norm that is spared counts.  Decode steps with a quantised
+// cache, norm and product / this, ms at 1 / 8 / 16 / 32 / 64 tokens: 24 layers of 1152 x 896 0.788 / 0.881 / 1.036 / 1.141 / 1.317 -> 0.762 /
+// 0.871 / 1.003 / 0.963 / 1.241; 28 of 4608 x 3584 at 1 / 8 / 16 2.88 / 3.08 / 3.37 and 2.91 / 3.03 / 3.37, 48 of 7168 x 5120 5.79 / 6.20 / 7.01
+// and 5.72 / 6.31 / 7.29.
+extern "C" int shk_few_plain_takes(int n, int m, int k) {
+  return n <= kFewTokens && m > 0 && m % 16 == 0 && k > 0 && k % 8 == 0 && static_cast<long long>(m) * k <= kFewHeadsMost;
+}
+
 extern "C" int shk_few_stream(const void* a, int lda, int n, int k, const void* wt, int m, const float* bias, float* resid,
                               const float* weight, void* rows, float* sums, void* stream) {
   FewRows x;
@@ -455,7 +470,7 @@ extern "C" int shk_few_heads(const void* a, int lda, int n, int k, const void* w
       few_heads_kernel<c.value, loads.value><<<dim3(groups, (n + 15) / 16), (waves + 1) * kWave, lds, static_cast<hipStream_t>(stream)>>>(
           x, static_cast<const u32x4*>(wt), kt, scaled, bias, static_cast<bf16*>(out), heads, kv_heads, head_dim, inv_freq, positions,
           token_seq, tables, table_stride, static_cast<bf16*>(k_pool), static_cast<bf16*>(v_pool), page_size, num_pages, write_kv,
-          magnitude);
+          magnitude, nullptr);
     });
   };
   if (sums)
@@ -463,5 +478,32 @@ extern "C" int shk_few_heads(const void* a, int lda, int n, int k, const void* w
   else
     go(std::integral_constant<int, 0>{});
   SHK_LAUNCH_CHECK("few_heads");
+  return 0;
+}
+
+extern "C" int shk_few_plain(const void* a, int lda, int n, int k, const void* wt, const float* sums, int count, float eps,
+                             const float* bias, float* out, int m, void* stream) {
+  FewRows x;
+  SHK_REQUIRE(few_rows_of(&x, a, lda, n, k, kFewTokens) && m > 0 && m % 16 == 0, "few_plain: bad sizes n=%d m=%d k=%d lda=%d", n, m, k, lda);
+  if (n == 0) return 0;
+  SHK_REQUIRE(a && wt && out, "few_plain: null pointer");
+  SHK_REQUIRE(reinterpret_cast<uintptr_t>(a) % 16 == 0, "few_plain: rows are not 16-byte aligned");
+  SHK_REQUIRE(!sums || (count > 0 && eps > 0.f), "few_plain: bad sums");
+  const FewScale scaled = {sums, count, 1.f / static_cast<float>(k), eps};
+  const int kt = (k + 31) / 32, waves = few_waves(kt, kFewTiles);
+  SHK_REQUIRE(!sums || count <= kFewMostLoads * (waves + 1) * 4, "few_plain: too many sums (%d)", count);
+  const auto go = [&](auto loads) {
+    with_tiles<kFewTiles>((kt + waves - 1) / waves, [&](auto c) {
+      const size_t lds = waves * kWave * sizeof(f32x4) + (waves + 1) * 16 * sizeof(float);
+      few_heads_kernel<c.value, loads.value><<<dim3(m / 16, (n + 15) / 16), (waves + 1) * kWave, lds, static_cast<hipStream_t>(stream)>>>(
+          x, static_cast<const u32x4*>(wt), kt, scaled, bias, nullptr, 0, 0, m, nullptr, nullptr, nullptr, nullptr, 0, nullptr, nullptr, 1, 0, 0,
+          1.f, out);
+    });
+  };
+  if (sums)
+    with_loads(count, (waves + 1) * kWave, go);
+  else
+    go(std::integral_constant<int, 0>{});
+  SHK_LAUNCH_CHECK("few_plain");
   return 0;
 }

@@ -61,9 +61,11 @@ _SIGNATURES = {
     "shk_few_stream_sums": [_I, _I, _I],
     "shk_few_gated_takes": [_I, _I, _I],
     "shk_few_heads_takes": [_I, _I, _I],
+    "shk_few_plain_takes": [_I, _I, _I],
     "shk_few_stream": [_P, _I, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P],
     "shk_few_gated": [_P, _I, _I, _I, _P, _P, _I, _F, _P, _P, _I, _I, _I, _P],
     "shk_few_heads": [_P, _I, _I, _I, _P, _P, _I, _F, _P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _F, _P],
+    "shk_few_plain": [_P, _I, _I, _I, _P, _P, _I, _F, _P, _P, _I, _P],
     "shk_mfma_alone": [_P, _P, _I, _I, _P],
     "shk_rope_kv_store": [_P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _P, _I, _I,
                           _F, _P],

@@ -581,6 +581,11 @@ def few_heads_takes(n: int, m: int, k: int) -> bool:
     return bool(load().shk_few_heads_takes(n, m, k))
 
 
+def few_plain_takes(n: int, m: int, k: int) -> bool:
+    """Whether few_plain takes n rows and an [m, k] matrix, and better than a product of normed rows."""
+    return bool(load().shk_few_plain_takes(n, m, k))
+
+
 def _few_rows(who, x, k, wt, numel, most=FEW_TOKENS):
     """(address, row stride, tokens) of rows [n, k], or [k / 8, n, 8] with the stride 0."""
     pieces = x.dim() == 3
@@ -620,6 +625,17 @@ def few_stream(a, wt, m: int, k: int, resid, weight, rows, sums, bias=None) -> N
         p, lda, n, k, _dev(wt, "wt"), m, None if bias is None else _dev(bias, "bias", torch.float32),
         _dev(resid, "resid", torch.float32), _dev(weight, "weight", torch.float32), _dev(rows, "rows"),
         _dev(sums, "sums", torch.float32), _stream()))
+
+
+def few_plain(x, wt, k: int, out, bias=None) -> None:
+    """The product of up to 64 rows (normed, or ScaledRows) with an [m, k] matrix, in float32: out [n, m]."""
+    rows, sums, count, eps = _few_sums("few_plain", x)
+    m = out.shape[-1]
+    p, lda, n = _few_rows("few_plain", rows, k, wt, tiled_numel(m, k))
+    if tuple(out.shape) != (n, m) or not out.is_contiguous() or (bias is not None and bias.numel() != m):
+        raise KernelError(f"few_plain: out must be contiguous [{n}, {m}], bias as wide")
+    check(load().shk_few_plain(p, lda, n, k, _dev(wt, "wt"), sums, count, eps, None if bias is None else _dev(bias, "bias", torch.float32),
+                               _dev(out, "out", torch.float32), m, _stream()))
 
 
 def few_gated(x: ScaledRows, wt, m: int, k: int, out, activation, gate_args=None) -> None:

@@ -724,11 +724,20 @@ class PagedAttention(Mixer):
         """Whether the step's projections, their rotation and the cache write are one kernel (ops.few_heads).  It leaves the
         queries alone beside the cache, so not for an attend() of another class, which may read the step's keys and values too."""
         s = self.spec
-        if not self.ends_onto or type(self).attend is not PagedAttention.attend or self.cache_dtype or self.plain_store or s.values_from_keys or self.position is None or getattr(self.position, "adjacent_pairs", False):
+        if self.cache_dtype:
+            return self._plain_rows(ctx)
+        if not self.ends_onto or type(self).attend is not PagedAttention.attend or self.plain_store or s.values_from_keys or self.position is None or getattr(self.position, "adjacent_pairs", False):
             return False
         table = self.position.rotary_table()
         return (table is not None and table[1] == s.head_dim and s.head_dim % 16 == 0 and self.w_qkv.tiled is not None
                 and ops.few_heads_takes(ctx.num_tokens, self.w_qkv.rows, self.width))
+
+    def _plain_rows(self, ctx) -> bool:
+        """The same with a quantised cache, whose write has to see a whole head: the projections (ops.few_plain) are a kernel and the write is one,
+        but the norm before them is none."""
+        return (self.ends_onto and type(self).attend is PagedAttention.attend
+                and (self.position is None or self.position.rotary_table() is not None) and self.w_qkv.tiled is not None
+                and ops.few_plain_takes(ctx.num_tokens, self.w_qkv.rows, self.width))
 
     def forward(self, ctx, x: torch.Tensor, cache) -> torch.Tensor:
         s = self.spec
@@ -753,7 +762,8 @@ class PagedAttention(Mixer):
             return self.linear_onto(ctx, "attn_proj", attn, self.w_o, bias=self.b_o)
         table = self.position.rotary_table() if self.position is not None else None
         tables = ctx.block_tables[cache.group]
-        if self.takes_scaled(ctx) and (isinstance(x, ops.ScaledRows) or ops.rows_aligned(x)):
+        few = self.takes_scaled(ctx) and (isinstance(x, ops.ScaledRows) or ops.rows_aligned(x))
+        if few and not self.cache_dtype:
             qkv = ctx.buffer("attn_qkv", (n, qkv_width), ctx.dtype)
             ops.few_heads(x, self.w_qkv.tiled, self.width, qkv, s.num_heads, s.num_kv_heads, s.head_dim, table[0], ctx.positions,
                           ctx.token_seq, tables, cache.pools["k"], cache.pools["v"], cache.page_size, write_kv=cache.owned,
@@ -763,7 +773,11 @@ class PagedAttention(Mixer):
             return self.linear_onto(ctx, "attn_proj", attn, self.w_o, bias=self.b_o)
         fused_position = self.position is None or table is not None
         split_sum = None
-        if fused_position:
+        if few:
+            sums = ctx.buffer("attn_qkv_sums", (1, n, qkv_width), torch.float32)
+            ops.few_plain(x, self.w_qkv.tiled, self.width, sums[0], bias=self.b_qkv)
+            split_sum, qkv = ops.SplitSum(sums), ctx.buffer("attn_qkv", (n, qkv_width), ctx.dtype)
+        elif fused_position:
             # the cache-write kernel can take the projections as partial sums
             qkv = self.linear_deferred(ctx, "attn_qkv_sum", x, self.w_qkv, bias=self.b_qkv,
                                        reader="position")
