@@ -95,11 +95,11 @@ __global__ void __launch_bounds__(kGeneralThreads)
 // Keys become bfloat16 with their power of two, values without: theirs joins the weight, before that is rounded to bfloat16 (an operand
 // of the matrix unit; maximum, sums and products stay float32).
 //
-// Many keys are bound by memory: 8 sequences of 16,000 keys, 40 heads of 128 over 8 (264 MB) 52 us, what a copy of as many bytes takes.
-// A wavefront has one chunk in flight and takes 1.4 us a chunk then; one sequence of 333 keys is one chunk a wavefront, 6.2 us, most of it
-// the way position -> page -> codes.  64 sequences of 61 to 4,000 keys 34 us where their bytes alone would take 26: they end at
-// different times.  Eight wavefronts a workgroup instead of four: 8 sequences of 2,060 keys of 4 heads 14.8 us unshared (16.3), and in the
-// shares that serve them best 11.6 (11.2); 128 of 100 to 900 22 (17).
+// Many keys are bound by memory: 8 sequences of 16,000 keys, 40 heads of 128 over 8 (264 MB) 51 us, what a copy of as many bytes takes.
+// A wavefront has one chunk in flight and takes 1.4 us a chunk then.  Few keys are bound by the way position -> page -> codes, 0.6 us a step, and by
+// fetching the instructions, which every launch does anew: one sequence of 333 keys 5.5 us.  64 sequences of 61 to 4,000 keys 34 us where
+// their bytes alone would take 26: they end at different times.  Eight wavefronts a workgroup instead of four: 8 sequences of 2,060 keys of 4 heads 14.8 us
+// unshared (16.3 then), and in the shares that served them best 11.6 (11.2); 128 of 100 to 900 22 (17).
 template <int D>
 struct KeyBlock {
   static constexpr int kPairs = D / 64, kOdd = D / 32 % 2;
@@ -147,7 +147,8 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
   int key_end = first + (z + 1) * per * 64;
   if (key_end > pos + 1) key_end = pos + 1;
 
-  // softmax state of head j, in base-2 logarithms; `l` is this lane's share of the sum until the end
+  // softmax state of head j, of the unscaled scores; `l` is this lane's share of the sum until the end
+  const float scale2 = scale * 1.4426950408889634f;  // base-2 logarithms
   float m = -INFINITY, l = 0.f;
   f32x4 o[D / 16];  // element db * 16 + 4 * g + r of head j
 #pragma unroll
@@ -166,7 +167,6 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
       }
       if (kOdd) qf[D / 32 - 1] = *reinterpret_cast<const bf16x8*>(row + kPairs * 64 + g * 8);
     }
-    const float scale2 = scale * 1.4426950408889634f;
     const int32_t* table = tables + static_cast<size_t>(seq) * table_stride;
     const size_t row_bytes = static_cast<size_t>(page_size) * D;
 
@@ -211,8 +211,7 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
       __builtin_amdgcn_sched_barrier(0);
     };
 
-    auto attend_chunk = [&](int kb, int next_kb, Pages next, auto edge_tag) {
-      constexpr bool edge = decltype(edge_tag)::value;
+    auto attend_chunk = [&](int kb, int next_kb, Pages next) {
       f32x4 s[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -233,11 +232,26 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
       const int g0 = kb + g * 16;
       float sc[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = s[e / 4][e % 4] * scale2;
-      if (edge) {
+      for (int e = 0; e < 16; ++e) sc[e] = s[e / 4][e % 4];
+      if (kb + 63 > pos || kb < lo) {  // wave-uniform
+        asm volatile("");  // (stays a branch: as a body of its own, which one wavefront runs, it took 1 us of a short launch to fetch)
+        // a slot that the query does not read may hold any byte: an infinite power of two, a NaN, and 0 times those would be NaN
+        u32x4 keep;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (g0 + e > pos || g0 + e < lo) sc[e] = -INFINITY;
+        for (int w = 0; w < 4; ++w) {
+          uint32_t bits = 0;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int e = 4 * w + b;
+            const bool out = g0 + e > pos || g0 + e < lo;
+            bits |= out ? 0u : 0xffu << (8 * b);
+            if (out) sc[e] = -INFINITY;
+          }
+          keep[w] = bits;
+        }
+        c.v_exp &= keep;
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db) c.v[db] &= keep;
       }
       float mx = max3(sc[0], sc[1], sc[2]);
 #pragma unroll
@@ -245,16 +259,14 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
       mx = lanes4_max(fmaxf(mx, sc[15]));
       const float m_new = fmaxf(m, mx);
       const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m - m_safe);
+      const float alpha = __builtin_amdgcn_exp2f((m - m_safe) * scale2), shift = -m_safe * scale2;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
       bf16x8 pf[2];
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float p = __builtin_amdgcn_exp2f(sc[e] - m_safe);
+        const float p = __builtin_amdgcn_exp2f(fmaf(sc[e], scale2, shift));
         sum[e % 4] += p;
-        float unit = __uint_as_float((c.v_exp[e / 4] >> (e % 4 * 8) & 0xffu) << 23);
-        // a slot that the query does not read may hold any byte: infinity, and 0 times that would be NaN
-        if (edge && (g0 + e > pos || g0 + e < lo)) unit = 0.f;
+        const float unit = __uint_as_float((c.v_exp[e / 4] >> (e % 4 * 8) & 0xffu) << 23);
         pf[e / 8][e % 8] = static_cast<__bf16>(p * unit);
       }
       l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
@@ -263,20 +275,9 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
 #pragma unroll
         for (int db = 0; db < D / 16; ++db) o[db] *= alpha;
       }
-      u32x4 keep = {~0u, ~0u, ~0u, ~0u};  // and its value any code, NaN among them
-      if (edge) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t bits = 0;
-#pragma unroll
-          for (int b = 0; b < 4; ++b) bits |= g0 + 4 * w + b > pos || g0 + 4 * w + b < lo ? 0u : 0xffu << (8 * b);
-          keep[w] = bits;
-        }
-      }
 #pragma unroll
       for (int db = 0; db < D / 16; ++db) {
-        u32x4 v = c.v[db];
-        if (edge) v &= keep;
+        const u32x4 v = c.v[db];
         o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(v[0], v[1], 1.f), pf[0], o[db], 0, 0, 0);
         o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(v[2], v[3], 1.f), pf[1], o[db], 0, 0, 0);
       }
@@ -291,10 +292,7 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
     next = find(clamped(key_begin + kStep));
     for (int kb = key_begin; kb < key_end; kb += kStep) {
       const Pages after = find(clamped(kb + 2 * kStep));
-      if (kb + 63 > pos || kb < lo)  // wave-uniform
-        attend_chunk(kb, clamped(kb + kStep), next, EdgeTag<true>{});
-      else
-        attend_chunk(kb, clamped(kb + kStep), next, EdgeTag<false>{});
+      attend_chunk(kb, clamped(kb + kStep), next);
       fetch_values(clamped(kb + kStep), next);
       next = after;
     }
@@ -313,8 +311,8 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
   const float m_ref = m_all == -INFINITY ? 0.f : m_all;
   l = 0.f;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) l += l_lds[w][j] * __builtin_amdgcn_exp2f(m_lds[w][j] - m_ref);  // 2^-inf = 0: nothing seen
-  const float mine = __builtin_amdgcn_exp2f(m - m_ref);
+  for (int w = 0; w < WAVES; ++w) l += l_lds[w][j] * __builtin_amdgcn_exp2f((m_lds[w][j] - m_ref) * scale2);  // 2^-inf = 0: nothing seen
+  const float mine = __builtin_amdgcn_exp2f((m - m_ref) * scale2);
 #pragma unroll
   for (int db = 0; db < D / 16; ++db) o_lds[wave][db][lane] = make_float4(o[db][0] * mine, o[db][1] * mine, o[db][2] * mine, o[db][3] * mine);
   __syncthreads();
@@ -343,7 +341,7 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
   // partial: O [row][share][D], then (maximum, sum) [row][share][2]
   if (nsplit > 1 && wave == 0 && g == 0)
     *reinterpret_cast<float2*>(partial + static_cast<size_t>(gridDim.y) * heads * nsplit * D + (head * nsplit + z) * 2) =
-        make_float2(m_all, l);
+        make_float2(m_all * scale2, l);
 }
 
 // out[row] = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z, shares in order: a wavefront per row (a token's head), lane z with share
@@ -373,13 +371,16 @@ __global__ void __launch_bounds__(kWave)
   float den = 0.f, acc[NE];
 #pragma unroll
   for (int e = 0; e < NE; ++e) acc[e] = 0.f;
+  // (lanes without a share have weight 0 and the last share's numbers)
+  auto of = [](float x, int z) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), z)); };
+  const float part = w * mine.y;
   for (int z0 = 0; z0 < nsplit; z0 += kBatch) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const float wz = z0 + u < nsplit ? __shfl(w, z0 + u, kWave) : 0.f;
-      den += z0 + u < nsplit ? __shfl(w * mine.y, z0 + u, kWave) : 0.f;
+      const float wz = of(w, z0 + u);
+      den += of(part, z0 + u);
 #pragma unroll
-      for (int e = 0; e < NE; ++e) acc[e] += wz * x[u][e];
+      for (int e = 0; e < NE; ++e) acc[e] = fmaf(wz, x[u][e], acc[e]);
     }
     if (z0 + kBatch < nsplit) fetch(z0 + kBatch);
   }

@@ -157,9 +157,9 @@ def decode_streams(num_seqs: int, kv_heads: int, head_dim: int, max_ctx: int, wi
 def e4m3_decode_splits(num_seqs: int, heads: int, kv_heads: int, head_dim: int, max_ctx: int) -> int:
     """Workgroups that share a single token's keys in a quantised cache: as many as put one on every compute unit, each with at
     least KEYS_PER_WORKGROUP keys for its four wavefronts; up to 512 keys none, where a second launch takes longer than the
-    wavefronts' second chunk (one sequence of 333, 14 heads of 64 over 2: 6.2 us, 7.6 in two).  28 heads of 128 over 4, us unshared / so:
-    one sequence of 2,000 14.4 / 9.0, 8 of 2,060 16.3 / 11.4; 40 over 8, 8 of 16,000 93 / 52; shares beyond a workgroup a unit lose what
-    joining them costs (64 sequences of 61 to 4,000 36 unshared, 38 in 4).  The batch is rounded up to a power of two, as it is padded
+    wavefronts' second chunk (one sequence of 333, 14 heads of 64 over 2: 5.5 us, 6.9 in two).  28 heads of 128 over 4, us unshared / so:
+    one sequence of 2,000 13.1 / 8.1, 8 of 2,060 15.2 / 11.1; 40 over 8, 8 of 16,000 89 / 51; shares beyond a workgroup a unit lose what
+    joining them costs (64 sequences of 61 to 4,000 34 unshared, 37 in 4).  The batch is rounded up to a power of two, as it is padded
     for graphs; so that a graph serves more than one length, prepare() rounds the longest context too."""
     if max_ctx <= 2 * KEYS_PER_WORKGROUP:
         return 1
@@ -175,9 +175,9 @@ E4M3_SHARE_KEYS = 128  # a turn of its two teams of wavefronts
 def e4m3_portion_splits(q_lens, starts, heads: int, kv_heads: int, head_dim: int, reach: int) -> int:
     """Workgroups that share the keys of a run of queries in a quantised cache (`reach`: the most keys that a query reads): as many
     as the launch leaves compute units for, each worth E4M3_SHARE_KEYS keys on average and KEYS_PER_WORKGROUP of the longest sequence's.
-    us unshared / so: 4 times 17 tokens at 700 to 1,900 of 14 heads of 64 over 2 27.7 / 13.6, 8 tokens at 2,000 of 28 of 128 over 4 35 /
-    15.3, 512 at 16,000 224 / 145 in 2; in twice as many 149, for the float32 results of a prompt's shares are large (2,048 at 0: 57
-    unshared, 92 in 2; two of 300 at 0, 16 over 16 15.5 and 21)."""
+    us unshared / so: 4 times 17 tokens at 700 to 1,900 of 14 heads of 64 over 2 25.8 / 13.1, 8 tokens at 2,000 of 28 of 128 over 4 35 /
+    15.5, 512 at 16,000 220 / 137 in 2; in twice as many 144, for the float32 results of a prompt's shares are large (2,048 at 0: 56
+    unshared, 91 in 2; two of 300 at 0, 16 over 16 15.4 and 21)."""
     queries = max(1, E4M3_ROWS // (heads // kv_heads))
     runs = longest = keys = total = 0
     for n, start in zip(q_lens, starts):
