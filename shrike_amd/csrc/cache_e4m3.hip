@@ -32,11 +32,11 @@ __device__ __forceinline__ void turn_of(int pos, float inv_freq, float magnitude
 
 __device__ __forceinline__ uint32_t size_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// A wavefront per head of a token, four neighbouring heads a workgroup; any sizes, types and ways of pairing.  A lane owns pairs that
-// turn together (lane, lane + 64) and elements behind the rotated part, forms its own cosines and meets nobody but its
+// A wavefront per head of a token, four neighbouring heads a workgroup; any sizes, types and ways of pairing.  A lane owns PAIRS pairs that
+// turn together (lane, lane + 64; one of heads of up to 128 elements) and elements behind the rotated part, forms its own cosines and meets nobody but its
 // wavefront: what a step of single tokens costs is the way of its loads.  (One workgroup per token, its heads one after the other, with
 // a table of cosines: 8 tokens of 28 heads over 4 11.1 us, 4.5 so.)
-template <typename T>
+template <typename T, int PAIRS>
 __global__ void __launch_bounds__(kStoreThreads) store_e4m3_kernel(StoreArgs a, E4m3Pools pools, int row_groups) {
   const int t = blockIdx.x / row_groups, lane = threadIdx.x % kWave;
   const int r = __builtin_amdgcn_readfirstlane(blockIdx.x % row_groups * kStoreWaves + threadIdx.x / kWave);
@@ -45,44 +45,19 @@ __global__ void __launch_bounds__(kStoreThreads) store_e4m3_kernel(StoreArgs a, 
   // heads of the queries, then of the keys, then of the values
   const bool value = r >= a.heads + a.kv_heads;
   const int from = (value && a.v_from_k ? r - a.kv_heads : r) * dim, turned = value ? 0 : a.rot_dim;
-  const int pos = a.positions[t];
+  const int pos = a.positions[t], seq = r >= a.heads ? a.token_seq[t] : 0;
   const T* row = static_cast<const T*>(a.qkv) + static_cast<size_t>(t) * width + from;
   const size_t stride = static_cast<size_t>(a.n) * width;
-  const float* part = a.parts + static_cast<size_t>(t) * width + from;
-  // columns d1 and d2 of the row; the parts of a split product are added in order, four of each in flight
-  auto get2 = [&](int d1, int d2, float& x1, float& x2) {
-    if (a.splits == 0) {
-      x1 = to_float(row[d1]);
-      x2 = to_float(row[d2]);
-      return;
-    }
-    x1 = x2 = 0.f;
-    for (int z0 = 0; z0 < a.splits; z0 += 4) {
-      float u[4], v[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const size_t at = stride * (z0 + k < a.splits ? z0 + k : a.splits - 1);
-        u[k] = part[at + d1];
-        v[k] = part[at + d2];
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        x1 += z0 + k < a.splits ? u[k] : 0.f;
-        x2 += z0 + k < a.splits ? v[k] : 0.f;
-      }
-    }
-    if (a.bias) {
-      x1 += a.bias[from + d1];
-      x2 += a.bias[from + d2];
-    }
-  };
-  // x[2 i], x[2 i + 1]: a pair that turns, or two elements that do not
-  constexpr int kPairs = kMaxDim / 2 / kWave;
-  float x[2 * kPairs];
-  int at[2 * kPairs];
+  const float* parts = a.parts + static_cast<size_t>(t) * width + from;
+  // x[2 i], x[2 i + 1]: a pair that turns, or two elements that do not.  Everything that does not hang on another load is asked for at
+  // once: the row (of a split product's parts the first four), its bias, the rates.
+  constexpr int kParts = 4;
   const int tail = (dim - turned + 1) / 2;  // pairs of elements that do not turn: d and d + tail
+  float x[2 * PAIRS], rate[PAIRS], bias[2 * PAIRS];
+  int at[2 * PAIRS], col[2 * PAIRS];
+  uint32_t raw[2 * PAIRS][kParts];
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
+  for (int i = 0; i < PAIRS; ++i) {
     const int p = lane + i * kWave;
     if (p < turned / 2) {
       at[2 * i] = a.adjacent ? 2 * p : p;
@@ -92,18 +67,57 @@ __global__ void __launch_bounds__(kStoreThreads) store_e4m3_kernel(StoreArgs a, 
       at[2 * i] = d < turned + tail ? d : dim;
       at[2 * i + 1] = d < turned + tail ? d + tail : dim;
     }
-    get2(min(at[2 * i], dim - 1), min(at[2 * i + 1], dim - 1), x[2 * i], x[2 * i + 1]);
+    col[2 * i] = min(at[2 * i], dim - 1), col[2 * i + 1] = min(at[2 * i + 1], dim - 1);
+    rate[i] = turned ? a.inv_freq[min(p, half - 1)] : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 2 * PAIRS; ++e) {
+    bias[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) raw[e][k] = 0;
+    if (a.splits == 0) {
+      if constexpr (sizeof(T) == 2)
+        raw[e][0] = reinterpret_cast<const uint16_t*>(row)[col[e]];
+      else
+        raw[e][0] = __float_as_uint(row[col[e]]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) raw[e][k] = __float_as_uint(parts[stride * min(k, a.splits - 1) + col[e]]);
+      if (a.bias) bias[e] = a.bias[from + col[e]];
+    }
   }
   int page = -1;
-  if (r >= a.heads)
-    page = e4m3_page(a.tables, a.table_stride, a.num_seqs, a.token_seq[t], pos, pools.page_size, pools.num_pages);
+  if (r >= a.heads) page = e4m3_page(a.tables, a.table_stride, a.num_seqs, seq, pos, pools.page_size, pools.num_pages);
+  if (a.splits == 0) {
+#pragma unroll
+    for (int e = 0; e < 2 * PAIRS; ++e) x[e] = __uint_as_float(sizeof(T) == 2 ? raw[e][0] << 16 : raw[e][0]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 2 * PAIRS; ++e) x[e] = 0.f;
+    for (int z0 = 0; z0 < a.splits; z0 += kParts) {  // added in order
+#pragma unroll
+      for (int e = 0; e < 2 * PAIRS; ++e)
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) x[e] += z0 + k < a.splits ? __uint_as_float(raw[e][k]) : 0.f;
+      if (z0 + kParts < a.splits) {
+#pragma unroll
+        for (int e = 0; e < 2 * PAIRS; ++e)
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) raw[e][k] = __float_as_uint(parts[stride * min(z0 + kParts + k, a.splits - 1) + col[e]]);
+      }
+    }
+    if (a.bias) {
+#pragma unroll
+      for (int e = 0; e < 2 * PAIRS; ++e) x[e] += bias[e];
+    }
+  }
   uint32_t largest = 0;
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
+  for (int i = 0; i < PAIRS; ++i) {
     const int p = lane + i * kWave;
     if (p < turned / 2) {
       float c, s;
-      turn_of(pos, a.inv_freq[p], a.magnitude, c, s);
+      turn_of(pos, rate[i], a.magnitude, c, s);
       const float x1 = x[2 * i], x2 = x[2 * i + 1];
       x[2 * i] = x1 * c - x2 * s;
       x[2 * i + 1] = x2 * c + x1 * s;
@@ -117,7 +131,7 @@ __global__ void __launch_bounds__(kStoreThreads) store_e4m3_kernel(StoreArgs a, 
   if (r < a.heads) {  // (all of the row has been read: it may be written in place)
     T* q_row = static_cast<T*>(a.q_out) + static_cast<size_t>(t) * a.q_ld + from;
 #pragma unroll
-    for (int e = 0; e < 2 * kPairs; ++e)
+    for (int e = 0; e < 2 * PAIRS; ++e)
       if (at[e] < dim) q_row[at[e]] = from_float<T>(x[e]);
     return;
   }
@@ -132,7 +146,7 @@ __global__ void __launch_bounds__(kStoreThreads) store_e4m3_kernel(StoreArgs a, 
   const size_t where = pools.part(page, r - a.heads - (value ? a.kv_heads : 0)), base = where * pools.row_bytes();
   if (lane == 0) pools.scales[(where * 2 + (value ? 1 : 0)) * pools.page_size + slot] = static_cast<uint8_t>(byte);
 #pragma unroll
-  for (int e = 0; e < 2 * kPairs; ++e) {
+  for (int e = 0; e < 2 * PAIRS; ++e) {
     if (at[e] >= dim) continue;
     const uint8_t code = e4m3_code(x[e], inverse, largest);
     if (value)
@@ -512,10 +526,9 @@ extern "C" int shk_rope_kv_store_e4m3(const void* qkv, int dtype, int n, int hea
     kernel<<<value_groups + n, kStoreThreads, 0, s>>>(a, pools, value_groups);
   } else {
     const int row_groups = (heads + (write_kv ? 2 * kv_heads : 0) + kStoreWaves - 1) / kStoreWaves;
-    if (dtype == kF32)
-      store_e4m3_kernel<float><<<n * row_groups, kStoreThreads, 0, s>>>(a, pools, row_groups);
-    else
-      store_e4m3_kernel<bf16><<<n * row_groups, kStoreThreads, 0, s>>>(a, pools, row_groups);
+    const auto kernel = head_dim <= 2 * kWave ? (dtype == kF32 ? store_e4m3_kernel<float, 1> : store_e4m3_kernel<bf16, 1>)
+                                              : (dtype == kF32 ? store_e4m3_kernel<float, 2> : store_e4m3_kernel<bf16, 2>);
+    kernel<<<n * row_groups, kStoreThreads, 0, s>>>(a, pools, row_groups);
   }
   SHK_LAUNCH_CHECK("rope_kv_store_e4m3");
   return 0;

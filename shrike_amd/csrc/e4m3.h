@@ -63,9 +63,10 @@ struct E4m3Pools {
 // The page of a sequence's token, -1 where there is none: a negative position, a sequence or position beyond the tables, an entry
 // outside the pool (a mistake of the caller's, never followed).
 __device__ __forceinline__ int e4m3_page(const int32_t* tables, int table_stride, int num_seqs, int seq, int pos, int page_size, int num_pages) {
-  if (pos < 0 || seq < 0 || seq >= num_seqs || pos / page_size >= table_stride) return -1;
-  const int page = tables[static_cast<size_t>(seq) * table_stride + pos / page_size];
-  return page >= 0 && page < num_pages ? page : -1;
+  const int entry = pos / page_size;
+  const bool there = pos >= 0 && seq >= 0 && seq < num_seqs && entry < table_stride;
+  const int page = tables[there ? static_cast<size_t>(seq) * table_stride + entry : 0];  // (no branch: nothing waits here)
+  return there && page >= 0 && page < num_pages ? page : -1;
 }
 
 }  // namespace shk
