@@ -351,6 +351,10 @@ __global__ void __launch_bounds__(kWave)
     merge_e4m3_kernel(const float* __restrict__ partial, bf16* __restrict__ out, int nsplit, const int32_t* __restrict__ cu_q,
                       int first_seq, int num_seqs, int heads) {
   constexpr int kBatch = 8, NE = (D + kWave - 1) / kWave;
+  // a lane's elements: neighbours where every lane has as many, so that they travel together
+  constexpr bool kNear = D % kWave == 0 && (NE & (NE - 1)) == 0;
+  typedef float Row __attribute__((ext_vector_type(NE)));
+  typedef __bf16 Out __attribute__((ext_vector_type(NE)));
   const size_t row = blockIdx.x;
   const int lane = threadIdx.x;
   const int token = first_seq + static_cast<int>(blockIdx.x / heads);
@@ -358,12 +362,18 @@ __global__ void __launch_bounds__(kWave)
   const float* src = partial + row * nsplit * D;
   float2 mine = make_float2(-INFINITY, 0.f);
   if (lane < nsplit) mine = *reinterpret_cast<const float2*>(partial + static_cast<size_t>(gridDim.x) * nsplit * D + (row * nsplit + lane) * 2);
-  float x[kBatch][NE];
+  Row x[kBatch];
   auto fetch = [&](int z0) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
+    for (int u = 0; u < kBatch; ++u) {
+      const float* share = src + static_cast<size_t>(min(z0 + u, nsplit - 1)) * D;
+      if constexpr (kNear) {
+        x[u] = *reinterpret_cast<const Row*>(share + lane * NE);
+      } else {
 #pragma unroll
-      for (int e = 0; e < NE; ++e) x[u][e] = src[static_cast<size_t>(min(z0 + u, nsplit - 1)) * D + min(lane + e * kWave, D - 1)];
+        for (int e = 0; e < NE; ++e) x[u][e] = share[min(lane + e * kWave, D - 1)];
+      }
+    }
   };
   fetch(0);
   const float mx = wave_max(mine.x);
@@ -386,9 +396,16 @@ __global__ void __launch_bounds__(kWave)
   }
   if (token < from || token >= to) return;
   const float inv = den == 0.f ? 0.f : 1.f / den;
+  if constexpr (kNear) {
+    Out y;
 #pragma unroll
-  for (int e = 0; e < NE; ++e)
-    if (lane + e * kWave < D) out[row * D + lane + e * kWave] = from_float<bf16>(acc[e] * inv);
+    for (int e = 0; e < NE; ++e) y[e] = static_cast<__bf16>(acc[e] * inv);
+    *reinterpret_cast<Out*>(out + row * D + lane * NE) = y;
+  } else {
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+      if (lane + e * kWave < D) out[row * D + lane + e * kWave] = from_float<bf16>(acc[e] * inv);
+  }
 }
 
 // ------------------------------------------------------------------ portions
