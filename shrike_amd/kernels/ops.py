@@ -829,8 +829,9 @@ def _e4m3_cache(who, kv_heads, head_dim, tables, k_pool, v_pool, scales, page_si
     if k_pool.dtype is not E4M3 or v_pool.dtype is not E4M3 or scales.dtype is not torch.uint8 or tables.dtype is not torch.int32:
         raise KernelError(f"{who}: pools must be float8_e4m3fn, scales uint8 and tables int32, got {k_pool.dtype}, {v_pool.dtype}, "
                           f"{scales.dtype} and {tables.dtype}")
-    pages = k_pool.shape[0]
-    if k_pool.shape != key_pool_shape(pages, kv_heads, page_size, head_dim):
+    shape, slab = k_pool.shape, key_slab(head_dim)
+    pages = shape[0]
+    if shape != (pages, kv_heads, head_dim // slab, page_size, slab):
         raise KernelError(f"{who}: key pool must be {list(key_pool_shape('pages', kv_heads, page_size, head_dim))}, "
                           f"got {tuple(k_pool.shape)}")
     if v_pool.shape != (pages, kv_heads, head_dim, page_size) or scales.shape != (pages, kv_heads, 2, page_size):
@@ -864,15 +865,20 @@ def rope_kv_store_e4m3(qkv, heads, kv_heads, head_dim, rot_dim, inv_freq, positi
     power of two of their own and rounded to E4M3, and that power's biased exponent goes to `scales`.  Angles are formed in
     float64.  q_out: rows [n, heads * head_dim] of qkv's dtype with unit inner stride that receive the queries (None: qkv's own query columns, in
     place; all of qkv's other columns stay as they are)."""
-    n = qkv.shape[0]
+    shape = qkv.shape
+    n = shape[0]
     width = (heads + (1 if values_from_keys else 2) * kv_heads) * head_dim
-    if qkv.dim() != 2 or not qkv.is_contiguous() or qkv.shape[1] != width:
+    if shape != (n, width) or not qkv.is_contiguous():
         raise KernelError("rope_kv_store_e4m3: qkv must be contiguous [n, (heads + 2 kv_heads) head_dim] "
                           "(heads + kv_heads with values_from_keys)")
+    q_step = width
     if q_out is None:
         q_out = qkv
-    elif q_out.dim() != 2 or q_out.stride(1) != 1 or q_out.shape != (n, heads * head_dim) or q_out.dtype != qkv.dtype:
-        raise KernelError("rope_kv_store_e4m3: q_out must be rows [n, heads * head_dim] of qkv's dtype with unit inner stride")
+    else:
+        steps = q_out.stride()
+        if q_out.shape != (n, heads * head_dim) or steps[1] != 1 or q_out.dtype is not qkv.dtype:
+            raise KernelError("rope_kv_store_e4m3: q_out must be rows [n, heads * head_dim] of qkv's dtype with unit inner stride")
+        q_step = steps[0]
     if rot_dim and (inv_freq is None or inv_freq.numel() < rot_dim // 2 or not inv_freq.is_contiguous()):
         raise KernelError(f"rope_kv_store_e4m3: a rotation of {rot_dim} elements needs {rot_dim // 2} frequencies")
     parts, splits, bias = None, 0, None
@@ -891,15 +897,15 @@ def rope_kv_store_e4m3(qkv, heads, kv_heads, head_dim, rot_dim, inv_freq, positi
         _dev(inv_freq, "inv_freq", torch.float32) if rot_dim else None, _step_rows("rope_kv_store_e4m3", n, positions),
         _step_rows("rope_kv_store_e4m3", n, token_seq) if write_kv else None, *cache, int(bool(write_kv)),
         None if parts is None else _dev(parts, "parts"), splits, None if bias is None else _dev(bias, "bias", torch.float32),
-        int(bool(adjacent_pairs)), int(bool(values_from_keys)), float(magnitude), _dev(q_out, "q_out"), q_out.stride(0), _stream()))
+        int(bool(adjacent_pairs)), int(bool(values_from_keys)), float(magnitude), _dev(q_out, "q_out"), q_step, _stream()))
 
 
 def kv_read_e4m3(k_out, v_out, kv_heads, head_dim, positions, token_seq, tables, k_pool, v_pool, scales, page_size) -> None:
     """Rows [n, kv_heads * head_dim] (float32 or bfloat16, which holds the values exactly) of the cached keys and values of the
     tokens at positions[t] of sequences token_seq[t]; NaN for a token that the tables do not have."""
-    n = k_out.shape[0]
-    if k_out.shape != (n, kv_heads * head_dim) or v_out.shape != k_out.shape or v_out.dtype != k_out.dtype \
-            or not (k_out.is_contiguous() and v_out.is_contiguous()):
+    shape = k_out.shape
+    n = shape[0]
+    if shape != (n, kv_heads * head_dim) or v_out.shape != shape or v_out.dtype is not k_out.dtype or not (k_out.is_contiguous() and v_out.is_contiguous()):
         raise KernelError("kv_read_e4m3: k_out and v_out must be contiguous [n, kv_heads * head_dim] of one dtype")
     check(load().shk_kv_read_e4m3(
         _dev(k_out, "k_out"), _dev(v_out, "v_out"), dtype_code(k_out.dtype), n, kv_heads, head_dim,
@@ -926,30 +932,42 @@ def attention_e4m3_supports_mfma(heads, kv_heads, head_dim, page_size, q_stride)
     return bool(load().shk_attention_e4m3_supports_mfma(heads, kv_heads, head_dim, page_size, q_stride))
 
 
-def _e4m3_rows(who, q, out, heads, head_dim, partial, rows, nsplit) -> int | None:
-    """Checks of the kernels on the matrix units; the scratch's address, None where there is one share."""
-    _rows(q, who + " q")
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+def _e4m3_rows(who, q, out, heads, head_dim, first, rows, partial, nsplit) -> tuple:
+    """Checks of the kernels on the matrix units, of `rows` rows from `first` on (None: all); addresses and stride (q, q_stride, out), the rows
+    of q, and the scratch's address (None where there is one share)."""
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16:
         raise KernelError(f"{who}: bfloat16 only")
-    if q.shape[1] < heads * head_dim or out.dim() != 2 or out.shape[1] != heads * head_dim or not out.is_contiguous():
+    have, step, to = q.shape, q.stride(), out.shape
+    if len(have) != 2 or step[1] != 1:
+        raise KernelError(f"{who} q: expected a 2-d tensor with unit inner stride")
+    width = heads * head_dim
+    if have[1] < width or len(to) != 2 or to[1] != width or not out.is_contiguous():
         raise KernelError(f"{who}: out must be contiguous rows of heads * head_dim, q at least as wide")
+    n = have[0]
+    if rows is None:
+        rows = n - first
+        if to[0] != n:
+            raise KernelError(f"{who}: out must have a row for each of q's")
+    elif n < rows or to[0] < rows:
+        raise KernelError(f"{who}: fewer rows than sequences")
+    if not (q.is_cuda and out.is_cuda):
+        raise KernelError(f"{who}: expected device tensors (there is no CPU path)")
+    at = (q.data_ptr(), step[0], out.data_ptr())
     if nsplit <= 1:
-        return None
-    need = rows * heads * nsplit * (head_dim + 2)
+        return at, n, None
+    need = rows * width * nsplit + 2 * rows * heads * nsplit
     if partial is None or partial.dtype != torch.float32 or not partial.is_contiguous() or partial.numel() < need:
         raise KernelError(f"{who}: {nsplit} shares of {rows} rows' keys need a contiguous float32 scratch of {need} values")
-    return _dev(partial, "partial")
+    return at, n, _dev(partial, "partial")
 
 
 def attention_decode_e4m3(q, out, num_seqs, heads, kv_heads, head_dim, positions, tables, k_pool, v_pool, scales, page_size, window, scale,
                           partial=None, nsplit: int = 1, chunk=None) -> None:
     """attention_decode() over a quantised cache: the first num_seqs rows of q, one token per sequence; nsplit workgroups share a
     token's keys, through `partial` (float32, num_seqs * heads * nsplit * (head_dim + 2) values) where they are more than one."""
-    scratch = _e4m3_rows("attention_decode_e4m3", q, out, heads, head_dim, partial, num_seqs, nsplit)
-    if q.shape[0] < num_seqs or out.shape[0] < num_seqs:
-        raise KernelError("attention_decode_e4m3: fewer rows than sequences")
+    rows, _, scratch = _e4m3_rows("attention_decode_e4m3", q, out, heads, head_dim, 0, num_seqs, partial, nsplit)
     check(load().shk_attention_decode_e4m3(
-        _dev(q, "q"), q.stride(0), _dev(out, "out"), num_seqs, heads, kv_heads, head_dim,
+        *rows, num_seqs, heads, kv_heads, head_dim,
         _step_rows("attention_decode_e4m3", num_seqs, positions),
         *_e4m3_cache("attention_decode_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size), int(window or 0),
         int(chunk or 0), float(scale), scratch, nsplit, _stream()))
@@ -961,12 +979,9 @@ def attention_prefill_e4m3(q, out, first_seq, num_seqs, heads, kv_heads, head_di
     first_seq + num_seqs - 1 (sequences before have one token each, which are not touched): rows cu_q[s] .. cu_q[s + 1], the last of
     ctx_lens[s] tokens.  nsplit workgroups share a run of queries' keys, through `partial` (float32, (rows of q - first_seq) * heads *
     nsplit * (head_dim + 2) values) where they are more than one."""
-    n = q.shape[0]
-    scratch = _e4m3_rows("attention_prefill_e4m3", q, out, heads, head_dim, partial, n - first_seq, nsplit)
-    if out.shape[0] != n:
-        raise KernelError("attention_prefill_e4m3: out must have a row for each of q's")
+    rows, n, scratch = _e4m3_rows("attention_prefill_e4m3", q, out, heads, head_dim, first_seq, None, partial, nsplit)
     check(load().shk_attention_prefill_e4m3(
-        _dev(q, "q"), q.stride(0), _dev(out, "out"), n, first_seq, num_seqs, heads, kv_heads, head_dim,
+        *rows, n, first_seq, num_seqs, heads, kv_heads, head_dim,
         _step_rows("attention_prefill_e4m3", first_seq + num_seqs + 1, cu_q),
         _step_rows("attention_prefill_e4m3", first_seq + num_seqs, ctx_lens),
         *_e4m3_cache("attention_prefill_e4m3", kv_heads, head_dim, tables, k_pool, v_pool, scales, page_size), int(window or 0),
