@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kWave)
 // The workgroups find their queries themselves, a sequence's last queries (which read the most keys) first, so a step needs no
 // lists from the host.
 //
-// 28 heads of 128 over 4: 512 tokens at 16,000 keys 136 us (880 TFLOP/s), 2,048 at 0 50 (600; with one team, conversions in a phase of
+// 28 heads of 128 over 4: 512 tokens at 16,000 keys 138 us (870 TFLOP/s), 2,048 at 0 50 (600; with one team, conversions in a phase of
 // their own and a reference that moves with every chunk: 513 and 135).  A turn of both teams, 128 keys, takes 2.1 to 2.4 us.  What bounds it: 44
 // operands of 16 bytes a lane and chunk out of LDS (1,400 cycles for the four wavefronts of a team, where their multiplications take
 // 1,150), instructions of any kind (with two wavefronts on a SIMD unit one every 5 cycles or so), and the clock, 1.9 GHz under this load.  Around
