@@ -37,9 +37,9 @@ __device__ __forceinline__ uint32_t size_bits(float x) { return __float_as_uint(
 // wavefront: what a step of single tokens costs is the way of its loads.  (One workgroup per token, its heads one after the other, with
 // a table of cosines: 8 tokens of 28 heads over 4 11.1 us, 4.3 so.)
 template <typename T, int PAIRS>
-__global__ void __launch_bounds__(kStoreThreads) store_e4m3_kernel(StoreArgs a, E4m3Pools pools, int row_groups) {
-  const int t = blockIdx.x / row_groups, lane = threadIdx.x % kWave;
-  const int r = __builtin_amdgcn_readfirstlane(blockIdx.x % row_groups * kStoreWaves + threadIdx.x / kWave);
+__global__ void __launch_bounds__(kStoreThreads) store_e4m3_kernel(StoreArgs a, E4m3Pools pools) {
+  const int t = blockIdx.x, lane = threadIdx.x % kWave;
+  const int r = __builtin_amdgcn_readfirstlane(blockIdx.y * kStoreWaves + threadIdx.x / kWave);
   const int dim = a.head_dim, half = a.rot_dim / 2, width = (a.heads + (a.v_from_k ? 1 : 2) * a.kv_heads) * dim;
   if (r >= a.heads + (a.write_kv ? 2 * a.kv_heads : 0)) return;
   // heads of the queries, then of the keys, then of the values
@@ -528,7 +528,7 @@ extern "C" int shk_rope_kv_store_e4m3(const void* qkv, int dtype, int n, int hea
     const int row_groups = (heads + (write_kv ? 2 * kv_heads : 0) + kStoreWaves - 1) / kStoreWaves;
     const auto kernel = head_dim <= 2 * kWave ? (dtype == kF32 ? store_e4m3_kernel<float, 1> : store_e4m3_kernel<bf16, 1>)
                                               : (dtype == kF32 ? store_e4m3_kernel<float, 2> : store_e4m3_kernel<bf16, 2>);
-    kernel<<<n * row_groups, kStoreThreads, 0, s>>>(a, pools, row_groups);
+    kernel<<<dim3(n, row_groups), kStoreThreads, 0, s>>>(a, pools);
   }
   SHK_LAUNCH_CHECK("rope_kv_store_e4m3");
   return 0;
