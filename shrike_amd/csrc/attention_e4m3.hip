@@ -349,19 +349,18 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
 template <int D>
 __global__ void __launch_bounds__(kWave)
     merge_e4m3_kernel(const float* __restrict__ partial, bf16* __restrict__ out, int nsplit, const int32_t* __restrict__ cu_q,
-                      int first_seq, int num_seqs, int heads) {
+                      int first_seq, int num_seqs) {
   constexpr int kBatch = 8, NE = (D + kWave - 1) / kWave;
   // a lane's elements: neighbours where every lane has as many, so that they travel together
   constexpr bool kNear = D % kWave == 0 && (NE & (NE - 1)) == 0;
   typedef float Row __attribute__((ext_vector_type(NE)));
   typedef __bf16 Out __attribute__((ext_vector_type(NE)));
-  const size_t row = blockIdx.x;
-  const int lane = threadIdx.x;
-  const int token = first_seq + static_cast<int>(blockIdx.x / heads);
+  const size_t row = static_cast<size_t>(blockIdx.x) * gridDim.y + blockIdx.y, rows = static_cast<size_t>(gridDim.x) * gridDim.y;
+  const int lane = threadIdx.x, token = first_seq + static_cast<int>(blockIdx.x);
   const int from = cu_q ? cu_q[first_seq] : 0, to = cu_q ? cu_q[first_seq + num_seqs] : token + 1;
   const float* src = partial + row * nsplit * D;
   float2 mine = make_float2(-INFINITY, 0.f);
-  if (lane < nsplit) mine = *reinterpret_cast<const float2*>(partial + static_cast<size_t>(gridDim.x) * nsplit * D + (row * nsplit + lane) * 2);
+  if (lane < nsplit) mine = *reinterpret_cast<const float2*>(partial + rows * nsplit * D + (row * nsplit + lane) * 2);
   Row x[kBatch];
   auto fetch = [&](int z0) {
 #pragma unroll
@@ -436,7 +435,7 @@ __global__ void __launch_bounds__(kWave)
 // their own and a reference that moves with every chunk: 513 and 135).  A turn of both teams, 128 keys, takes 2.1 to 2.4 us.  What bounds it: 44
 // operands of 16 bytes a lane and chunk out of LDS (1,400 cycles for the four wavefronts of a team, where their multiplications take
 // 1,150), instructions of any kind (with two wavefronts on a SIMD unit one every 5 cycles or so), and the clock, 1.9 GHz under this load.  Around
-// the turns 4.5 us until the first multiplication (sequence -> page -> codes -> LDS) and 2 us to join and leave, which is most of a
+// the turns 4 us until the first multiplication (sequence -> page -> codes -> LDS) and 2 us to join and leave, which is most of a
 // short portion: 4 of 17 tokens at 700 to 1,900 keys 11 us.  Keeping codes in LDS instead would spare 16 of the 44 reads, but every wavefront
 // would convert the whole chunk, 96 instructions more.
 constexpr int kPortionRows = 128;
@@ -449,8 +448,8 @@ struct PortionArgs {
   const int32_t *cu_q, *ctx_lens, *tables;
   const uint8_t *k_pool, *v_pool, *scales;
   float* partial;
-  int n, q_stride, heads, kv_heads, queries, first_seq, num_seqs, table_stride, page_size, num_pages, window, block, nsplit;
-  uint32_t page_magic;
+  int n, q_stride, heads, kv_heads, group, queries, first_seq, num_seqs, table_stride, page_size, num_pages, window, block, nsplit;
+  uint32_t page_magic, group_magic, queries_magic;  // ceil(2^32 / page_size), ceil(2^16 / group), ceil(2^32 / queries)
   float scale;
 };
 
@@ -470,17 +469,21 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
   const int col = lane % 32, half = lane / 32;
   const int page_size = PAGE ? PAGE : a.page_size;
   const PageDiv pd{page_size, a.page_magic};
-  const int z = blockIdx.x % a.nsplit, kvh = blockIdx.x / a.nsplit % a.kv_heads;
+  // grid (key/value head, share, run), and the runs beyond 65,535 behind the shares: no division, of which each costs thirty instructions
+  // that a short launch fetches to run once
+  const int kvh = blockIdx.x;
+  int z = blockIdx.y, left = blockIdx.z;
+  for (; z >= a.nsplit; z -= a.nsplit) left += gridDim.z;
 
   // ---- this workgroup's sequence and first query: lane i looks at sequence i, so that one round of loads finds everything
-  const int group = a.heads / a.kv_heads;
+  const int group = a.group;
   int seq = -1, q0 = 0, tok0 = 0, tok1 = 0, ctx = 0;
   {
-    int left = blockIdx.x / (a.nsplit * a.kv_heads);
     for (int base = 0; base < a.num_seqs; base += kWave) {
       const int i = a.first_seq + min(base + lane, a.num_seqs - 1);
       const int from = a.cu_q[i], to = a.cu_q[i + 1], length = a.ctx_lens[i];
-      const int runs = base + lane < a.num_seqs && to > from ? (to - from + a.queries - 1) / a.queries : 0;
+      const uint32_t up = to - from + a.queries - 1;
+      const int runs = base + lane < a.num_seqs && to > from ? static_cast<int>(a.queries == 1 ? up : __umulhi(up, a.queries_magic)) : 0;
       int upto = runs;
 #pragma unroll
       for (int off = 1; off < kWave; off <<= 1) {
@@ -517,7 +520,8 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
   const int c_end = c_first + per_split < nchunks ? c_first + per_split : nchunks;
 
   // the lane's row (both halves of the wavefront hold the same 32, both teams all of them); a lane without one reads no key
-  const int row = member * 32 + col, qi = q0 + row / group, head = kvh * group + row % group;
+  const int row = member * 32 + col, qrow = static_cast<int>(row * a.group_magic >> 16);  // row / group
+  const int qi = q0 + qrow, head = kvh * group + row - qrow * group;
   const bool mine = row < a.queries * group && qi < q_end;
   const int q_pos = mine ? start + qi : -1, q_lo = first_key(q_pos, a.window, a.block);
   bf16x8 qf[KS];
@@ -979,9 +983,9 @@ bool aligned16(const void* a, const void* b, const void* c) {
 uint32_t page_magic(int page_size) { return static_cast<uint32_t>(((1ull << 32) + page_size - 1) / page_size); }
 
 template <int D>
-void merge_e4m3(int rows, hipStream_t s, const float* partial, void* out, int nsplit, const int32_t* cu_q = nullptr, int first_seq = 0,
-                int num_seqs = 0, int heads = 1) {
-  merge_e4m3_kernel<D><<<rows, kWave, 0, s>>>(partial, static_cast<bf16*>(out), nsplit, cu_q, first_seq, num_seqs, heads);
+void merge_e4m3(int tokens, int heads, hipStream_t s, const float* partial, void* out, int nsplit, const int32_t* cu_q = nullptr,
+                int first_seq = 0, int num_seqs = 0) {
+  merge_e4m3_kernel<D><<<dim3(tokens, heads), kWave, 0, s>>>(partial, static_cast<bf16*>(out), nsplit, cu_q, first_seq, num_seqs);
 }
 
 #define E4M3_BY_DIM(head_dim, CASE) \
@@ -999,8 +1003,8 @@ void merge_e4m3(int rows, hipStream_t s, const float* partial, void* out, int ns
 }  // namespace
 
 extern "C" int shk_attention_e4m3_supports_mfma(int heads, int kv_heads, int head_dim, int page_size, int q_stride) {
-  return heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 128 && head_dim >= 32 && head_dim <= 256 &&
-         head_dim % 32 == 0 && page_size > 0 && page_size % 16 == 0 && q_stride >= heads * head_dim && q_stride % 8 == 0;
+  return heads > 0 && heads <= 65535 && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 128 && head_dim >= 32 &&
+         head_dim <= 256 && head_dim % 32 == 0 && page_size > 0 && page_size % 16 == 0 && q_stride >= heads * head_dim && q_stride % 8 == 0;
 }
 
 extern "C" int shk_attention_decode_e4m3(const void* q, int q_stride, void* out, int num_seqs, int heads, int kv_heads, int head_dim,
@@ -1025,7 +1029,7 @@ extern "C" int shk_attention_decode_e4m3(const void* q, int q_stride, void* out,
       static_cast<const bf16*>(q), q_stride, static_cast<bf16*>(out), heads, head_tiles, positions, tables, table_stride,        \
       static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(scales), kv_heads,   \
       page_size, page_magic(page_size), num_pages, window, chunk, scale, partial, nsplit);                                       \
-  if (nsplit > 1) merge_e4m3<D>(num_seqs * heads, s, partial, out, nsplit)
+  if (nsplit > 1) merge_e4m3<D>(num_seqs, heads, s, partial, out, nsplit)
   E4M3_BY_DIM(head_dim, LAUNCH)
 #undef LAUNCH
   SHK_LAUNCH_CHECK("attention_decode_e4m3");
@@ -1050,22 +1054,23 @@ extern "C" int shk_attention_prefill_e4m3(const void* q, int q_stride, void* out
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int tokens = n - first_seq, group = heads / kv_heads;
   const int queries = kPortionRows / group;
-  const long long count = static_cast<long long>(tokens / queries + num_seqs) * kv_heads * nsplit;
-  SHK_REQUIRE(count < (1LL << 31) && static_cast<long long>(tokens) * heads < (1LL << 31), "attention_prefill_e4m3: too many tokens: %d",
-              tokens);
+  const long long runs = static_cast<long long>(tokens) / queries + num_seqs, deep = runs < 65535 ? runs : 65535, layers = (runs + deep - 1) / deep;
+  SHK_REQUIRE(tokens < (1 << 25) && layers * nsplit <= 65535 && static_cast<long long>(tokens) * heads < (1LL << 31),
+              "attention_prefill_e4m3: too many tokens: %d", tokens);
   SHK_REQUIRE(static_cast<long long>(num_pages) * kv_heads < (1LL << 31) && static_cast<long long>(page_size) * head_dim < (1LL << 31),
               "attention_prefill_e4m3: %d pages of %d are too many", num_pages, page_size);
   const PortionArgs a{static_cast<const bf16*>(q), static_cast<bf16*>(out), cu_q, ctx_lens, tables, static_cast<const uint8_t*>(k_pool),
                       static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(scales), partial, n, q_stride, heads, kv_heads,
-                      queries, first_seq, num_seqs, table_stride, page_size, num_pages, window, chunk, nsplit,
-                      page_magic(page_size), scale};
+                      group, queries, first_seq, num_seqs, table_stride, page_size, num_pages, window, chunk, nsplit,
+                      page_magic(page_size), static_cast<uint32_t>((65536 + group - 1) / group), page_magic(queries), scale};
+  const dim3 grid(kv_heads, static_cast<unsigned>(layers) * nsplit, static_cast<unsigned>(deep));
 #define LAUNCH(D)                                                                                                       \
   constexpr int kTeams##D = D <= 128 ? 2 : 1;                                                                           \
   (page_size == 16 ? attention_portion_e4m3_kernel<D, kTeams##D, 16> : attention_portion_e4m3_kernel<D, kTeams##D, 0>)   \
-      <<<static_cast<unsigned>(count), kTeams##D * 4 * kWave, 0, s>>>(a);                                               \
+      <<<grid, kTeams##D * 4 * kWave, 0, s>>>(a);                                                                       \
   if (nsplit > 1)                                                                                                        \
-  merge_e4m3<D>(tokens * heads, s, partial, static_cast<bf16*>(out) + static_cast<size_t>(first_seq) * heads * D, nsplit, cu_q, \
-                first_seq, num_seqs, heads)
+  merge_e4m3<D>(tokens, heads, s, partial, static_cast<bf16*>(out) + static_cast<size_t>(first_seq) * heads * D, nsplit, cu_q, \
+                first_seq, num_seqs)
   E4M3_BY_DIM(head_dim, LAUNCH)
 #undef LAUNCH
   SHK_LAUNCH_CHECK("attention_prefill_e4m3");

@@ -385,3 +385,35 @@ def test_refusals_of_what_is_not_aligned(ops):
             ops.attention_decode_e4m3(q, args[0], 1, heads, kv, dim, *single, args[1], 2)
         with pytest.raises(KernelError, match="aligned"):
             ops.attention_prefill_e4m3(q, args[0], 1, 1, heads, kv, dim, *runs, args[1], 2)
+
+
+@pytest.mark.parametrize("news", [[1] * 70, [300, 1, 129, 2], [128] * 9])
+@pytest.mark.parametrize("form", [(64, 1, 32, 16), (128, 1, 32, 16), (3, 1, 64, 16), (2, 2, 64, 16)])
+def test_runs_of_queries_of_every_length(ops, form, news):
+    """Groups that do not divide 128, runs of one query, sequences that end inside a run and with it."""
+    heads, kv, dim, ps = form
+    step = plain.Step([(37 * i) % 90 for i in range(len(news))], news, ps, seed=11)
+    pools, keys, values, q = setup(step, form)
+    for nsplit in (1, 3):
+        out = torch.full((step.n, heads * dim), 9.0, dtype=torch.bfloat16, device="cuda")
+        partial = torch.empty(step.n * heads * nsplit * (dim + 2), device="cuda")
+        ops.attention_prefill_e4m3(q.cuda(), out, 0, len(news), heads, kv, dim, step.cu_q.cuda(), step.ctx_lens.cuda(), step.tables.cuda(),
+                                   *pools, ps, None, dim ** -0.5, partial, nsplit)
+        check(step, form, out, q, keys, values, None, None)
+
+
+def test_more_runs_than_a_grid_is_deep(ops):
+    """70,000 runs of one query: the same bits as in two calls."""
+    form = heads, kv, dim, ps = 128, 1, 32, 16
+    step = plain.Step([0] * 700, [100] * 700, ps, seed=12)
+    k_pool, v_pool, scales, _, _ = plain.random_pools(step.pages, kv, dim, ps, step.gen)
+    pools = (k_pool.cuda(), v_pool.cuda(), scales.cuda())
+    q = torch.randn(step.n, heads * dim, device="cuda").bfloat16()
+    cu_q, ctx_lens, tables = step.cu_q.cuda(), step.ctx_lens.cuda(), step.tables.cuda()
+    whole, halves = (torch.full_like(q, 9.0) for _ in range(2))
+    ops.attention_prefill_e4m3(q, whole, 0, 700, heads, kv, dim, cu_q, ctx_lens, tables, *pools, ps, None, dim ** -0.5)
+    for first in (0, 350):
+        rows = slice(100 * first, 100 * first + 35000)
+        ops.attention_prefill_e4m3(q[rows], halves[rows], 0, 350, heads, kv, dim, cu_q[:351], ctx_lens[first:first + 350],
+                                   tables[first:first + 350], *pools, ps, None, dim ** -0.5)
+    assert whole.isfinite().all() and torch.equal(whole, halves) and not (whole == 9.0).all(1).any()
