@@ -4,11 +4,11 @@ state of fixed size.
 
 Layers whose mixers ask for the same PagedSpec form a group; a group has its
 own pool of pages, its own device tensors (whatever the spec lists per page,
-each as ``[layers, pages + 1, *its shape for one page]``: what a page holds and
-how it is laid out is the mixer's business, not the manager's) and, per request,
-its own block table.  A group with a window or a block-local mask gives pages back
-as soon as no later query can reach them (table entry -1); all pages come back when
-the request ends.
+each as ``[layers, pages + 1, *its shape for one page]``, a layer's part beginning
+on 16 bytes: what a page holds and how it is laid out is the mixer's business, not
+the manager's) and, per request, its own block table.  A group with a window or a
+block-local mask gives pages back as soon as no later query can reach them (table
+entry -1); all pages come back when the request ends.
 Layers whose mixers ask for a StateSpec form state groups: a tensor
 ``[layers, slots, *shape]`` indexed by the request's state slot.  Every request
 holds one slot, whether or not any layer has state.
@@ -20,6 +20,7 @@ shrike/engine/model_runner.py:52-60, which is one group without a window.
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 
 from ..parts.base import CompositeSpec, PagedSpec, StateSpec
@@ -70,6 +71,17 @@ class StateGroup:
         self.layers: list[int] = []
         self.tensor = None  # [layers, slots, *shape]
         self.padded = None  # [layers, slots + 1, *shape], the same memory plus the spare slot
+
+
+def _aligned_layers(layers: int, shape: tuple, dtype, device):
+    """Zeros [layers, *shape] whose layers are contiguous and begin on 16 bytes each: kernels move that much of a page
+    at a time, and one byte a token, or an odd number of elements, times an odd number of pages ends anywhere."""
+    import torch
+
+    numel = math.prod(shape)
+    step = 16 // torch.empty(0, dtype=dtype).element_size()
+    rows = torch.zeros(layers, -(-numel // step) * step, dtype=dtype, device=device)
+    return rows[:, :numel].view(layers, *shape)
 
 
 class CacheManager:
@@ -146,9 +158,9 @@ class CacheManager:
             # one page more than the pool hands out: page `num_pages` is where the
             # padding rows of a fixed-size (graph) batch put what they write
             for t in g.spec.tensors:
-                g.tensors[t.name] = torch.zeros(
-                    len(g.layers), self.num_pages + 1, *t.shape(self.page_size),
-                    dtype=dtype if t.dtype is None else getattr(torch, t.dtype), device=device,
+                g.tensors[t.name] = _aligned_layers(
+                    len(g.layers), (self.num_pages + 1, *t.shape(self.page_size)),
+                    dtype if t.dtype is None else getattr(torch, t.dtype), device,
                 )
         for g in self.state_groups:
             g.padded = torch.zeros(
