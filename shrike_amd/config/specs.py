@@ -640,6 +640,18 @@ class ModelSpec:
                         f"schedule[{pos}] reads the cache of position {entry.cache_of}, "
                         "which does not own one"
                     )
+                kept, own = (_cache_dtypes(self.blocks[self.schedule[i].block].mixer) for i in (entry.cache_of, pos))
+                for name in kept.keys() & own.keys():
+                    if kept[name] != own[name]:
+                        raise ValueError(
+                            f"schedule[{pos}] keeps its keys and values in {own[name] or 'the compute dtype'} and reads the "
+                            f"cache of position {entry.cache_of}, which is in {kept[name] or 'the compute dtype'}"
+                        )
+
+
+def _cache_dtypes(mixer) -> dict:
+    """AttentionSpec.cache_dtype of a mixer and of its branches, by sub-name ("" without branches)."""
+    return {name: getattr(m, "cache_dtype", None) for name, m in getattr(mixer, "branches", (("", mixer),))}
 
 
 def with_cache_dtype(spec: ModelSpec, cache_dtype: str | None) -> ModelSpec:
