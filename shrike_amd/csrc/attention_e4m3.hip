@@ -259,12 +259,13 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
       mx = lanes4_max(fmaxf(mx, sc[15]));
       const float m_new = fmaxf(m, mx);
       const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f((m - m_safe) * scale2), shift = -m_safe * scale2;
+      const float alpha = __builtin_amdgcn_exp2f((m - m_safe) * scale2);
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
       bf16x8 pf[2];
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(sc[e], scale2, shift));
+        // (not fma(score, scale2, -m_safe scale2): of scores beyond 2^31 that product's rounding alone over- or underflows)
+        const float p = __builtin_amdgcn_exp2f((sc[e] - m_safe) * scale2);
         sum[e % 4] += p;
         const float unit = __uint_as_float((c.v_exp[e / 4] >> (e % 4 * 8) & 0xffu) << 23);
         pf[e / 8][e % 8] = static_cast<__bf16>(p * unit);
@@ -341,15 +342,15 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
   // partial: O [row][share][D], then (maximum, sum) [row][share][2]
   if (nsplit > 1 && wave == 0 && g == 0)
     *reinterpret_cast<float2*>(partial + static_cast<size_t>(gridDim.y) * heads * nsplit * D + (head * nsplit + z) * 2) =
-        make_float2(m_all * scale2, l);
+        make_float2(m_all, l);
 }
 
-// out[row] = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z, shares in order: a wavefront per row (a token's head), lane z with share
+// out[row] = sum_z w_z O_z / sum_z w_z l_z, w_z = 2^((m_z - M) scale2), shares in order: a wavefront per row (a token's head), lane z with share
 // z's weight.  With `cu_q` a row counts only if its token is one of the sequences': there are no shares of the others.
 template <int D>
 __global__ void __launch_bounds__(kWave)
-    merge_e4m3_kernel(const float* __restrict__ partial, bf16* __restrict__ out, int nsplit, const int32_t* __restrict__ cu_q,
-                      int first_seq, int num_seqs) {
+    merge_e4m3_kernel(const float* __restrict__ partial, bf16* __restrict__ out, int nsplit, float scale2,
+                      const int32_t* __restrict__ cu_q, int first_seq, int num_seqs) {
   constexpr int kBatch = 8, NE = (D + kWave - 1) / kWave;
   // a lane's elements: neighbours where every lane has as many, so that they travel together
   constexpr bool kNear = D % kWave == 0 && (NE & (NE - 1)) == 0;
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(kWave)
   };
   fetch(0);
   const float mx = wave_max(mine.x);
-  const float w = mine.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine.x - mx);
+  const float w = mine.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mine.x - mx) * scale2);
   float den = 0.f, acc[NE];
 #pragma unroll
   for (int e = 0; e < NE; ++e) acc[e] = 0.f;
@@ -441,6 +442,7 @@ __global__ void __launch_bounds__(kWave)
 constexpr int kPortionRows = 128;
 constexpr float kSlack = 10.f;  // log2 of the largest weight relative to the reference: beyond it moves
 constexpr int kMostUnit = 40;
+constexpr float kFarShift = 8192.f;  // log2: rounding the reference times the scale moves weights by up to 2^-12 below it
 
 struct PortionArgs {
   const bf16* q;
@@ -823,10 +825,23 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
     }
+    float by = shift;
+    if (__builtin_amdgcn_ballot_w64(fabsf(shift) > kFarShift) != 0) {
+      // (kept a branch) of scores beyond 2^31 that rounding alone would make every weight infinite or 0: here the reference leaves
+      // the scores before they are scaled
+      asm volatile("");
+      const bool large = fabsf(shift) > kFarShift;
+      const float ref = large ? m : 0.f;
+      by = large ? 0.f : shift;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[t][e] -= ref;
+    }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[u][e] = static_cast<__bf16>(__builtin_amdgcn_exp2f(fmaf(s[u / 2][u % 2 * 8 + e], scale2, shift)));
+      for (int e = 0; e < 8; ++e) p[u][e] = static_cast<__bf16>(__builtin_amdgcn_exp2f(fmaf(s[u / 2][u % 2 * 8 + e], scale2, by)));
   };
 
   if (c_first < c_end) {  // the same for every wavefront of the workgroup
@@ -911,7 +926,7 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
 #pragma unroll
     for (int i = 0; i < kMine; ++i) *reinterpret_cast<f32x4*>(dst + i * 8) = sums[i];
     if (!half && team == 0)
-      *reinterpret_cast<float2*>(a.partial + rows * a.nsplit * D + (at * a.nsplit + z) * 2) = make_float2(m * scale2, total);
+      *reinterpret_cast<float2*>(a.partial + rows * a.nsplit * D + (at * a.nsplit + z) * 2) = make_float2(m, total);
     return;
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;  // (a query that reads no key: zeros)
@@ -983,9 +998,10 @@ bool aligned16(const void* a, const void* b, const void* c) {
 uint32_t page_magic(int page_size) { return static_cast<uint32_t>(((1ull << 32) + page_size - 1) / page_size); }
 
 template <int D>
-void merge_e4m3(int tokens, int heads, hipStream_t s, const float* partial, void* out, int nsplit, const int32_t* cu_q = nullptr,
+void merge_e4m3(int tokens, int heads, hipStream_t s, const float* partial, void* out, int nsplit, float scale, const int32_t* cu_q = nullptr,
                 int first_seq = 0, int num_seqs = 0) {
-  merge_e4m3_kernel<D><<<dim3(tokens, heads), kWave, 0, s>>>(partial, static_cast<bf16*>(out), nsplit, cu_q, first_seq, num_seqs);
+  merge_e4m3_kernel<D><<<dim3(tokens, heads), kWave, 0, s>>>(partial, static_cast<bf16*>(out), nsplit, scale * 1.4426950408889634f, cu_q,
+                                                            first_seq, num_seqs);
 }
 
 #define E4M3_BY_DIM(head_dim, CASE) \
@@ -1029,7 +1045,7 @@ extern "C" int shk_attention_decode_e4m3(const void* q, int q_stride, void* out,
       static_cast<const bf16*>(q), q_stride, static_cast<bf16*>(out), heads, head_tiles, positions, tables, table_stride,        \
       static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(scales), kv_heads,   \
       page_size, page_magic(page_size), num_pages, window, chunk, scale, partial, nsplit);                                       \
-  if (nsplit > 1) merge_e4m3<D>(num_seqs, heads, s, partial, out, nsplit)
+  if (nsplit > 1) merge_e4m3<D>(num_seqs, heads, s, partial, out, nsplit, scale)
   E4M3_BY_DIM(head_dim, LAUNCH)
 #undef LAUNCH
   SHK_LAUNCH_CHECK("attention_decode_e4m3");
@@ -1069,8 +1085,8 @@ extern "C" int shk_attention_prefill_e4m3(const void* q, int q_stride, void* out
   (page_size == 16 ? attention_portion_e4m3_kernel<D, kTeams##D, 16> : attention_portion_e4m3_kernel<D, kTeams##D, 0>)   \
       <<<grid, kTeams##D * 4 * kWave, 0, s>>>(a);                                                                       \
   if (nsplit > 1)                                                                                                        \
-  merge_e4m3<D>(tokens, heads, s, partial, static_cast<bf16*>(out) + static_cast<size_t>(first_seq) * heads * D, nsplit, cu_q, \
-                first_seq, num_seqs)
+  merge_e4m3<D>(tokens, heads, s, partial, static_cast<bf16*>(out) + static_cast<size_t>(first_seq) * heads * D, nsplit, scale, \
+                cu_q, first_seq, num_seqs)
   E4M3_BY_DIM(head_dim, LAUNCH)
 #undef LAUNCH
   SHK_LAUNCH_CHECK("attention_prefill_e4m3");
