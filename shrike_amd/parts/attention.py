@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import numpy as np
@@ -60,8 +61,6 @@ def distance_buckets(rows: int, reach: int) -> list[int]:
     with half = rows // 2, the distances below half have a row each; from there on the row is half
     + floor(ln(d / half) / ln(reach / half) * (rows - half)), the rest of the rows spread evenly over
     the logarithm of the distance up to `reach`; the last row serves that distance and all beyond."""
-    import math
-
     half = rows // 2
     out = []
     for d in range(reach + 1):
@@ -166,6 +165,12 @@ def e4m3_decode_splits(num_seqs: int, heads: int, kv_heads: int, head_dim: int, 
     tiles = kv_heads * -(-heads // (16 * kv_heads))
     want = -(-compute_units() // (_pow2(num_seqs) * tiles))
     return max(1, min(want, -(-max_ctx // KEYS_PER_WORKGROUP), MAX_KEY_SPLITS))
+
+
+def _e4m3_matrix_scale(scale: float) -> bool:
+    """Whether the quantised cache's kernels on the matrix units take a scale (they add exponents over it to scores);
+    ops.attention_e4m3 takes every other one."""
+    return 2.0 ** -100 <= scale <= 2.0 ** 100
 
 
 E4M3_ROWS = 128  # rows (queries times heads of a key/value head) a workgroup of the quantised cache's prompt kernel
@@ -431,7 +436,7 @@ class PagedAttention(Mixer):
         s = self.spec
         if self.cache_dtype not in (None, "e4m3"):
             raise ValueError(f"{self.name}: cache_dtype must be None or e4m3, got {self.cache_dtype!r}")
-        if self.cache_dtype and (self.plain_store or not s.scale > 0):
+        if self.cache_dtype and (self.plain_store or not 0 < s.scale < math.inf):
             raise ValueError(f"{self.name}: a cache in {self.cache_dtype} is built for attention that rotates its keys or stores them as "
                              "they are, with values of their size and a positive scale")
         if self.plain_store:
@@ -514,7 +519,8 @@ class PagedAttention(Mixer):
         s = self.spec
         return ("paged_attention", s.num_heads, s.num_kv_heads, s.head_dim, s.window, s.chunk, self.plain_store,
                 self.talking, self.value_dim, self._qkv_width(), bool(getattr(s, "bucket_bias", None)),
-                bool(getattr(s, "softcap", None)), bool(getattr(s, "sinks", False)), bool(self.cache_dtype))
+                bool(getattr(s, "softcap", None)), bool(getattr(s, "sinks", False)), bool(self.cache_dtype),
+                bool(self.cache_dtype) and _e4m3_matrix_scale(s.scale))
 
     def context_scratch_bytes(self, rows: int, keys: int) -> int:
         s = self.spec
@@ -534,7 +540,8 @@ class PagedAttention(Mixer):
         plan = shape.notes[key] = AttentionPlan()
         if self.cache_dtype:
             # the portions' kernel finds its workgroups' queries itself: no lists
-            plan.mfma = self.dtype == torch.bfloat16 and ops.attention_e4m3_supports_mfma(h, hkv, d, shape.page_size, self._qkv_width())
+            plan.mfma = (self.dtype == torch.bfloat16 and _e4m3_matrix_scale(s.scale)
+                         and ops.attention_e4m3_supports_mfma(h, hkv, d, shape.page_size, self._qkv_width()))
             if plan.mfma:
                 reach = min(x for x in (s.window, s.chunk, 1 << 40) if x)
                 if shape.num_decode:
