@@ -17,6 +17,18 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
+// x / page_size and x % page_size for every x >= 0 without a division: with 2^(L-1) < page_size <= 2^L the magic number ceil(2^(31+L) / page_size)
+// fits 32 bits and is off by less than 1, so x * magic by less than 2^31 of the 2^(31+L) that are one.  (PageDiv has no shift, and is for
+// x < 2^32 / page_size alone: positions of long contexts lie beyond where pages are large.)
+struct AnyPageDiv {
+  int ps;
+  uint32_t magic;
+  __device__ __forceinline__ int div(int x) const {
+    return static_cast<int>(__umulhi(static_cast<uint32_t>(x), magic) >> (31 - __builtin_clz(ps - 1)));
+  }
+  __device__ __forceinline__ int mod(int x) const { return x - div(x) * ps; }
+};
+
 constexpr int kMaxShares = 64;  // workgroups that share a query's keys: a lane of the kernel that joins them each
 constexpr int kGeneralThreads = 256, kGeneralDim = 256;
 
@@ -138,7 +150,7 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1)
   const int first_head = kvh * group + blockIdx.x % head_tiles * 16;  // of this workgroup's tile
   const int tile_heads = min(16, kvh * group + group - first_head);
   const int page_size = PAGE ? PAGE : any_page_size;
-  const PageDiv pd{page_size, page_magic};
+  const AnyPageDiv pd{page_size, page_magic};
   const int pos = positions[seq], lo = first_key(pos, window, block);
   const int first = lo & ~63;
   const int chunks = pos < 0 ? 0 : (pos - first) / 64 + 1;
@@ -451,7 +463,7 @@ struct PortionArgs {
   const uint8_t *k_pool, *v_pool, *scales;
   float* partial;
   int n, q_stride, heads, kv_heads, group, queries, first_seq, num_seqs, table_stride, page_size, num_pages, window, block, nsplit;
-  uint32_t page_magic, group_magic, queries_magic;  // ceil(2^32 / page_size), ceil(2^16 / group), ceil(2^32 / queries)
+  uint32_t page_magic, group_magic, queries_magic;  // of AnyPageDiv; ceil(2^16 / group), ceil(2^32 / queries)
   float scale;
 };
 
@@ -470,7 +482,7 @@ __global__ void __launch_bounds__(TEAMS * 4 * kWave, TEAMS) attention_portion_e4
   const int team = wave / 4, member = wave % 4;
   const int col = lane % 32, half = lane / 32;
   const int page_size = PAGE ? PAGE : a.page_size;
-  const PageDiv pd{page_size, a.page_magic};
+  const AnyPageDiv pd{page_size, a.page_magic};
   // grid (key/value head, share, run), and the runs beyond 65,535 behind the shares: no division, of which each costs thirty instructions
   // that a short launch fetches to run once
   const int kvh = blockIdx.x;
@@ -995,7 +1007,9 @@ bool aligned16(const void* a, const void* b, const void* c) {
   return (reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) % 16 == 0;
 }
 
-uint32_t page_magic(int page_size) { return static_cast<uint32_t>(((1ull << 32) + page_size - 1) / page_size); }
+uint32_t page_magic(int page_size) {
+  return static_cast<uint32_t>(((1ull << (63 - __builtin_clz(page_size - 1))) + page_size - 1) / page_size);
+}
 
 template <int D>
 void merge_e4m3(int tokens, int heads, hipStream_t s, const float* partial, void* out, int nsplit, float scale, const int32_t* cu_q = nullptr,
@@ -1078,7 +1092,8 @@ extern "C" int shk_attention_prefill_e4m3(const void* q, int q_stride, void* out
   const PortionArgs a{static_cast<const bf16*>(q), static_cast<bf16*>(out), cu_q, ctx_lens, tables, static_cast<const uint8_t*>(k_pool),
                       static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(scales), partial, n, q_stride, heads, kv_heads,
                       group, queries, first_seq, num_seqs, table_stride, page_size, num_pages, window, chunk, nsplit,
-                      page_magic(page_size), static_cast<uint32_t>((65536 + group - 1) / group), page_magic(queries), scale};
+                      page_magic(page_size), static_cast<uint32_t>((65536 + group - 1) / group),
+                      static_cast<uint32_t>(((1ull << 32) + queries - 1) / queries), scale};
   const dim3 grid(kv_heads, static_cast<unsigned>(layers) * nsplit, static_cast<unsigned>(deep));
 #define LAUNCH(D)                                                                                                       \
   constexpr int kTeams##D = D <= 128 ? 2 : 1;                                                                           \
