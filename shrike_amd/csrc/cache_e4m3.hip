@@ -7,7 +7,13 @@ namespace shk {
 
 constexpr int kStoreThreads = 256, kStoreWaves = kStoreThreads / kWave;
 constexpr int kMaxDim = 256;
-constexpr int kManyTokens = 65;
+// From how many tokens on, and wavefronts of the kernel for few of them, its rows travel in vectors: where a wavefront per head no longer fits
+// the chip at once (32 on each of 256 compute units; heads of more than 128 elements count twice).  us a wavefront per head / in vectors:
+// 14 heads of 64 over 2 at 128 / 384 / 512 tokens 4.1 / 5.6 / 6.5 and 5.7 / 5.9 / 5.9, 28 of 128 over 4 at 128 / 192 / 256 4.9 / 5.6 / 6.3 and 6.0 /
+// 6.1 / 6.1, 40 over 8 at 96 / 128 / 160 5.2 / 5.6 / 6.4 and 6.0 / 6.1 / 6.1, 112 over 8 at 65 / 80 / 128 6.1 / 6.8 / 8.5 and 7.0 / 7.1 / 7.3, 8 of 256
+// over 1 at 384 / 512 5.8 / 6.2 and 6.3 / 6.3.  In four parts with a bias the two meet at up to twice as many tokens where heads are many
+// (112 over 8 at 192 / 256 14.3 / 17.8 and 15.3 / 16.7), else at as many (28 over 4 at 192 / 256 6.4 / 7.5 and 6.6 / 6.9).
+constexpr int kManyTokens = 65, kManyWaves = 256 * 32;
 
 struct StoreArgs {
   const void* qkv;      // [n, width], or null with parts
@@ -519,7 +525,8 @@ extern "C" int shk_rope_kv_store_e4m3(const void* qkv, int dtype, int n, int hea
   const E4m3Pools pools{static_cast<uint8_t*>(k_pool), static_cast<uint8_t*>(v_pool), static_cast<uint8_t*>(scales), page_size,
                         num_pages, kv_heads, head_dim};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (n >= kManyTokens && dtype == kBF16 && rot_dim == head_dim && head_dim % 32 == 0 && !pairing && !v_from_k && q_ld % 8 == 0 &&
+  const long long waves = static_cast<long long>(n) * (heads + (write_kv ? 2LL * kv_heads : 0)) * (head_dim <= 2 * kWave ? 1 : 2);
+  if (n >= kManyTokens && waves > kManyWaves && dtype == kBF16 && rot_dim == head_dim && head_dim % 32 == 0 && !pairing && !v_from_k && q_ld % 8 == 0 &&
       reinterpret_cast<uintptr_t>(splits ? static_cast<const void*>(parts) : qkv) % 16 == 0 && reinterpret_cast<uintptr_t>(q_out) % 16 == 0) {
     const unsigned value_groups = write_kv ? static_cast<unsigned>((n + kBlock - 1) / kBlock * kv_heads) : 0;
     const auto kernel = head_dim <= 64 ? store_many_e4m3_kernel<4> : head_dim <= 128 ? store_many_e4m3_kernel<8> : store_many_e4m3_kernel<16>;
