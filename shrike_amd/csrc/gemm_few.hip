@@ -384,9 +384,13 @@ extern "C" int shk_few_heads_takes(int n, int m, int k) {
 // Rows that a kernel of their own rotates and stores: small matrices alone, where the norm that is spared counts.  Decode steps with a quantised
 // cache, norm and product / this, ms at 1 / 8 / 16 / 32 / 64 tokens: 24 layers of 1152 x 896 0.788 / 0.881 / 1.036 / 1.141 / 1.317 -> 0.762 /
 // 0.871 / 1.003 / 0.963 / 1.241; 28 of 4608 x 3584 at 1 / 8 / 16 2.88 / 3.08 / 3.37 and 2.91 / 3.03 / 3.37, 48 of 7168 x 5120 5.79 / 6.20 / 7.01
-// and 5.72 / 6.31 / 7.29.
+// and 5.72 / 6.31 / 7.29.  us that a layer gains (twelve of them at 100 to 200 keys): 1536 x 1024 0.9 / 1.0 / 0.7 / 3.7 / 2.0, 1792 x 1280 2.1 /
+// 2.8 / 0.4 / 0.4 / 0.1, 2048 x 1536 0.0 / 0.3 / -0.6 / 0.0 / -0.9, 2560 x 2048 -0.5 / -0.8 / -1.1 / -1.3 / -2.7, 2816 x 2304 0.0 / -0.3 / -0.5 / -1.5 / -3.4.
+// Up to 16 tokens the line is few_heads' (between 2048 x 1536 and 2816 x 2304 this is up to 1.1 us a layer too much); of more, whose every 16 read the
+// weights again, it lies where nothing is gained any more.
+constexpr long long kFewPlainMost = 2500 * 1000;
 extern "C" int shk_few_plain_takes(int n, int m, int k) {
-  return n <= kFewTokens && m > 0 && m % 16 == 0 && k > 0 && k % 8 == 0 && static_cast<long long>(m) * k <= kFewHeadsMost;
+  return n <= kFewTokens && m > 0 && m % 16 == 0 && k > 0 && k % 8 == 0 && static_cast<long long>(m) * k <= (n <= 16 ? kFewHeadsMost : kFewPlainMost);
 }
 
 extern "C" int shk_few_stream(const void* a, int lda, int n, int k, const void* wt, int m, const float* bias, float* resid,
