@@ -40,7 +40,9 @@ class EngineConfig:
     cache_dtype: None keeps keys and values in the compute dtype; "e4m3" (or "fp8") as 8-bit codes
         with a power of two per token and head: half the bytes of bfloat16 and twice the tokens in
         the same memory, for models whose every layer is attention that rotates its keys or
-        stores them as they are (others are refused).
+        stores them as they are (others are refused).  For bfloat16 with heads of a multiple of 32
+        elements and pages of a multiple of 16 tokens; what else there is, float32 among it, is
+        served by a kernel for any sizes, 10 to 13 times as slow as attention over a float32 cache.
     graphs: replay decode-only steps from HIP graphs.
     overlap_steps: launch the next decode step before the host has read the
         tokens of this one (they pass from the sampler to the next step on the

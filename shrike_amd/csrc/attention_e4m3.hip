@@ -1,5 +1,8 @@
 // Attention over a quantised key/value cache (e4m3.h).  A code times its power of two is a bfloat16 number, so what is
-// attended over is exactly what the cache stands for; scores, softmax statistics and sums are float32 everywhere.
+// attended over is exactly what the cache stands for; scores, softmax statistics and sums are float32 everywhere.  On the matrix
+// units a weight is rounded to bfloat16 before it meets the values, as in the kernels over the bfloat16 cache: 2^-8 of it at most, what
+// rounding the result costs too (results are off from 64 bits by 1.6e-3 to 2.0e-3 of their size, with float32 weights by 1.6e-3 or 1.7e-3).
+// Single tokens' denominators add up the weights before that, portions' the rounded ones.  The kernel for any sizes rounds none.
 //
 // attention_e4m3_kernel: any head size up to 256, any page size and group, float32 or bfloat16 queries; one workgroup per
 // (token, head).  What the kernels on the matrix units do not take.
@@ -33,7 +36,10 @@ constexpr int kMaxShares = 64;  // workgroups that share a query's keys: a lane 
 constexpr int kGeneralThreads = 256, kGeneralDim = 256;
 
 // Keys in runs of 256 from the query's first key on, a thread per key for its score, a thread per (part of the run, element)
-// for the values; running maximum and sum.
+// for the values; running maximum and sum, in one order whatever else the step holds.  It is made for any size, not for speed: codes
+// come byte by byte, a head's group reads its keys head by head, and nobody shares a token's keys.  14 heads of 64 over 2 in float32: one
+// sequence of 2,000 keys 174 us, 8 of 2,060 188, a prompt of 512 324, where the kernels over a float32 cache take 17, 18 and 27; 28 of 128 over 4
+// 327, 372, 1232 (24, 32, 120); in bfloat16 16 of 80 over 4 195, 231, 330, pages of 8 tokens 28 of 128 over 4 312, 379, 1070.
 template <typename T>
 __global__ void __launch_bounds__(kGeneralThreads)
     attention_e4m3_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, int heads,
@@ -109,7 +115,7 @@ __global__ void __launch_bounds__(kGeneralThreads)
 //
 // Many keys are bound by memory: 8 sequences of 16,000 keys, 40 heads of 128 over 8 (264 MB) 51 us, what a copy of as many bytes takes.
 // A wavefront has one chunk in flight and takes 1.4 us a chunk then.  Few keys are bound by the way position -> page -> codes, 0.6 us a step, and by
-// fetching the instructions, which every launch does anew: one sequence of 333 keys 5.5 us.  64 sequences of 61 to 4,000 keys 34 us where
+// fetching the instructions, which every launch does anew: one sequence of 333 keys 5.0 us.  64 sequences of 61 to 4,000 keys 33 us where
 // their bytes alone would take 26: they end at different times.  Eight wavefronts a workgroup instead of four: 8 sequences of 2,060 keys of 4 heads 14.8 us
 // unshared (16.3 then), and in the shares that served them best 11.6 (11.2); 128 of 100 to 900 22 (17).
 template <int D>
@@ -451,6 +457,10 @@ __global__ void __launch_bounds__(kWave)
 // the turns 4 us until the first multiplication (sequence -> page -> codes -> LDS) and 2 us to join and leave, which is most of a
 // short portion: 4 of 17 tokens at 700 to 1,900 keys 11 us.  Keeping codes in LDS instead would spare 16 of the 44 reads, but every wavefront
 // would convert the whole chunk, 96 instructions more.
+//
+// Heads of more than 128 elements: two teams' chunks do not fit LDS, so there is one, whose conversions overlap with nothing.  512 tokens at
+// 16,000 / 2,048 at 0, from graphs: 16 heads of 160 over 2 134 / 66 us (640 / 320 TFLOP/s), 16 of 192 over 4 144 / 73, 16 of 224 over 2 167 / 83, 16 of 256
+// over 4 181 / 92 (750 / 370), 8 over 1 102 / 63.
 constexpr int kPortionRows = 128;
 constexpr float kSlack = 10.f;  // log2 of the largest weight relative to the reference: beyond it moves
 constexpr int kMostUnit = 40;

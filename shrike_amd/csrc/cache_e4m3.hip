@@ -41,7 +41,9 @@ __device__ __forceinline__ uint32_t size_bits(float x) { return __float_as_uint(
 // A wavefront per head of a token, four neighbouring heads a workgroup; any sizes, types and ways of pairing.  A lane owns PAIRS pairs that
 // turn together (lane, lane + 64; one of heads of up to 128 elements) and elements behind the rotated part, forms its own cosines and meets nobody but its
 // wavefront: what a step of single tokens costs is the way of its loads.  (One workgroup per token, its heads one after the other, with
-// a table of cosines: 8 tokens of 28 heads over 4 11.1 us, 4.3 so.)
+// a table of cosines: 8 tokens of 28 heads over 4 11.1 us, 4.3 so.)  Many tokens come here too where the kernel below does not take them, and
+// their codes leave byte by byte: 8,192 of 40 heads of 128 over 8 turned by neighbours 167 us, half of each head 165, values from keys 167, not at
+// all 122, in float32 201, heads of 80 165, where that kernel takes 41 (all from graphs).
 template <typename T, int PAIRS>
 __global__ void __launch_bounds__(kStoreThreads) store_e4m3_kernel(StoreArgs a, E4m3Pools pools) {
   const int t = blockIdx.x, lane = threadIdx.x % kWave;

@@ -158,7 +158,7 @@ def e4m3_decode_splits(num_seqs: int, heads: int, kv_heads: int, head_dim: int, 
     least KEYS_PER_WORKGROUP keys for its four wavefronts; up to 512 keys none, where a second launch takes longer than the
     wavefronts' second chunk (one sequence of 333, 14 heads of 64 over 2: 5.5 us, 6.9 in two).  28 heads of 128 over 4, us unshared / so:
     one sequence of 2,000 13.1 / 8.1, 8 of 2,060 15.2 / 11.1; 40 over 8, 8 of 16,000 89 / 51; shares beyond a workgroup a unit lose what
-    joining them costs (64 sequences of 61 to 4,000 34 unshared, 37 in 4).  The batch is rounded up to a power of two, as it is padded
+    joining them costs (64 sequences of 61 to 4,000 34 unshared, 37 in 4).  `head_dim` does not count.  The batch is rounded up to a power of two, as it is padded
     for graphs; so that a graph serves more than one length, prepare() rounds the longest context too."""
     if max_ctx <= 2 * KEYS_PER_WORKGROUP:
         return 1
@@ -182,7 +182,9 @@ def e4m3_portion_splits(q_lens, starts, heads: int, kv_heads: int, head_dim: int
     as the launch leaves compute units for, each worth E4M3_SHARE_KEYS keys on average and KEYS_PER_WORKGROUP of the longest sequence's.
     us unshared / so: 4 times 17 tokens at 700 to 1,900 of 14 heads of 64 over 2 25.8 / 13.1, 8 tokens at 2,000 of 28 of 128 over 4 35 /
     15.5, 512 at 16,000 220 / 137 in 2; in twice as many 144, for the float32 results of a prompt's shares are large (2,048 at 0: 56
-    unshared, 91 in 2; two of 300 at 0, 16 over 16 15.4 and 21)."""
+    unshared, 91 in 2; two of 300 at 0, 16 over 16 15.4 and 21).  `head_dim` does not count, though heads of more than 128 elements have
+    a turn of 64 keys: of 512 tokens at 16,000 the rule's shares are the fastest there too (16 of 256 over 4 337 / 181 / 195 in 2 / 4 / 8, 4 the rule's),
+    of 2,048 at 0 it is 6 to 12 % behind twice as many (83 in 2, 92), of 4 times 17 at 1,000 15 % (23 in 4, 20 in 8)."""
     queries = max(1, E4M3_ROWS // (heads // kv_heads))
     runs = longest = keys = total = 0
     for n, start in zip(q_lens, starts):
