@@ -263,7 +263,7 @@ int shk_qkv_store(void* qkv, int dtype, int n, int heads, int kv_heads, int head
 // Queries go to q_out, rows q_ld elements apart (qkv itself, q_ld its width: in place).  Tokens that are not there leave the pools alone.
 // A call holds a position of a sequence once, and no page that another call running at the same time writes.
 // shk_kv_read_e4m3: rows [n, kv_heads * head_dim] of `dtype` of the tokens (token_seq[t], positions[t]); NaN for one that is not there.
-// shk_attention_e4m3: shk_attention over such a cache (window, chunk; no cap, sinks or bias); scale > 0.  Keys that are not there
+// shk_attention_e4m3: shk_attention over such a cache (window, chunk; no cap, sinks or bias), up to 65,535 tokens; scale > 0.  Keys that are not there
 // are not read; a query without any key gets zeros.
 int shk_rope_kv_store_e4m3(const void* qkv, int dtype, int n, int heads, int kv_heads, int head_dim, int rot_dim,
                            const float* inv_freq, const int32_t* positions, const int32_t* token_seq, const int32_t* tables,
@@ -279,7 +279,7 @@ int shk_attention_e4m3(const void* q, int q_stride, void* out, int dtype, int n,
                        int chunk, float scale, void* stream);
 
 // The same on the matrix units for bfloat16, where shk_attention_e4m3_supports_mfma says so (head_dim a multiple of 32 up to 256,
-// page_size of 16, up to 128 query heads a key/value head, q rows 16-byte aligned; out and partial are too).  Here every key that a
+// page_size of 16, up to 128 query heads a key/value head, q rows 16-byte aligned; out and partial are too), scale from 2^-100 to 2^100.  Here every key that a
 // query reads has to be there: a page outside the pool or the tables is not followed, but another one is read in its place.
 // shk_attention_decode_e4m3: sequence s has one query token, row s of q, at positions[s]; nsplit > 1 workgroups share its keys.
 // shk_attention_prefill_e4m3: rows first_seq .. n - 1 of q and out are the new tokens of sequences first_seq .. first_seq +

@@ -915,7 +915,8 @@ def kv_read_e4m3(k_out, v_out, kv_heads, head_dim, positions, token_seq, tables,
 
 def attention_e4m3(q, out, heads, kv_heads, head_dim, positions, token_seq, tables, k_pool, v_pool, scales, page_size, window, scale,
                    chunk=None) -> None:
-    """attention() over a quantised cache, any sizes: q [n, >= heads * head_dim] rows of float32 or bfloat16, out [n, heads * head_dim]."""
+    """attention() over a quantised cache, any sizes: q [n, >= heads * head_dim] rows of float32 or bfloat16, up to 65,535 of them, out
+    [n, heads * head_dim]."""
     _rows(q, "attention_e4m3 q")
     n = q.shape[0]
     if q.shape[1] < heads * head_dim or out.shape != (n, heads * head_dim) or not out.is_contiguous() or out.dtype != q.dtype:
@@ -928,7 +929,7 @@ def attention_e4m3(q, out, heads, kv_heads, head_dim, positions, token_seq, tabl
 
 
 def attention_e4m3_supports_mfma(heads, kv_heads, head_dim, page_size, q_stride) -> bool:
-    """Whether attention_decode_e4m3 and attention_prefill_e4m3 take these sizes; attention_e4m3 takes all."""
+    """Whether attention_decode_e4m3 and attention_prefill_e4m3 take these sizes (with scales from 2^-100 to 2^100); attention_e4m3 takes all."""
     return bool(load().shk_attention_e4m3_supports_mfma(heads, kv_heads, head_dim, page_size, q_stride))
 
 
